@@ -1,0 +1,71 @@
+"""What the 4-bit and 8-bit operators refuse before they launch anything, and what a launch without a device returns; no GPU is needed."""
+import pytest
+import torch
+from ctypes import c_float, c_int, c_longlong, c_void_p
+
+from transformer_amd import kernels
+
+AT = c_void_p(1 << 20)
+
+
+def _gemm(lib, M=4, N=64, K=64, x=AT, codes=AT, ldx=None, ldo=None, dtype=1, glu=0):
+    return lib.ta_gemm_mx4(None, c_int(dtype), c_int(glu), x, c_longlong(K if ldx is None else ldx), codes, AT, None, AT,
+                           c_longlong(N if ldo is None else ldo), c_int(M), c_int(N), c_int(K))
+
+
+def _gemm8(lib, M=4, N=64, K=64, x=AT, ldo=None):
+    return lib.ta_gemm_mx4_mx8(None, x, AT, AT, AT, None, AT, c_longlong(N if ldo is None else ldo), c_int(M), c_int(N), c_int(K))
+
+
+def _refused(rc, name):
+    lib = kernels.library()
+    assert rc != 0 and lib.ta_last_error().startswith(name) and b"launch failed" not in lib.ta_last_error(), lib.ta_last_error()
+
+
+def test_products_refuse_what_their_kernels_do_not_take():
+    lib = kernels.library()
+    off = c_void_p((1 << 20) + 8)
+    for kw in (dict(K=48), dict(K=0), dict(M=-1), dict(N=0), dict(x=off), dict(codes=off), dict(ldx=68), dict(ldx=32), dict(ldo=63), dict(dtype=2),
+               dict(M=65), dict(N=1 << 30, glu=1)):
+        _refused(_gemm(lib, **kw), b"ta_gemm_mx4:")
+    for kw in (dict(K=48), dict(M=-1), dict(N=0), dict(x=off), dict(ldo=63), dict(M=2147483647, N=2147483647)):
+        _refused(_gemm8(lib, **kw), b"ta_gemm_mx4_mx8:")
+    assert lib.ta_mx4_max_rows() == kernels.MX4_MAX_ROWS
+    assert _gemm(lib, M=0) == 0 and _gemm8(lib, M=0) == 0
+
+
+def test_rows_refuse_what_their_kernels_do_not_take():
+    lib = kernels.library()
+    off, ll = c_void_p((1 << 20) + 4), c_longlong
+    for k, ld, p, dtype in ((48, 48, AT, 0), (64, 60, AT, 0), (64, 66, AT, 0), (64, 68, AT, 1), (64, 64, off, 0), (64, 64, AT, 2)):
+        for name in ("ta_mx4_pack", "ta_mx8_pack"):
+            _refused(getattr(lib, name)(None, c_int(dtype), p, ll(ld), AT, AT, ll(3), c_int(k)), name.encode())
+        _refused(lib.ta_mx4_unpack(None, c_int(dtype), AT, AT, p, ll(ld), ll(3), c_int(k)), b"ta_mx4_unpack")
+    for d, ld, p, bias, dtype in ((48, 96, AT, None, 0), (64, 124, AT, None, 0), (64, 130, AT, None, 0), (64, 132, AT, None, 1), (64, 128, off, None, 0),
+                                  (64, 128, AT, off, 0), (64, 128, AT, None, 2)):
+        _refused(lib.ta_swiglu_mx8(None, c_int(dtype), p, ll(ld), bias, AT, AT, ll(3), c_int(d)), b"ta_swiglu_mx8")
+    _refused(lib.ta_mx8_pack(None, c_int(0), AT, ll(1 << 20), AT, AT, ll(1 << 40), c_int(1 << 20)), b"ta_mx8_pack")
+
+    def norm(n=3, d=64, planes=0, delta=None, to=AT, bias=None, x=AT, dtype=0):
+        return lib.ta_add_rmsnorm_mx8(None, c_int(dtype), x, delta, c_int(planes), bias, AT, c_float(1e-5), to, AT, AT, c_int(n), c_int(d))
+    for kw in (dict(d=48), dict(n=-1), dict(planes=1), dict(delta=AT), dict(planes=9, delta=AT), dict(planes=1, delta=AT, to=None), dict(bias=AT, to=None),
+               dict(x=off), dict(dtype=2)):
+        _refused(norm(**kw), b"ta_add_rmsnorm_mx8:")
+
+
+def test_tensors_off_the_gpu_are_refused():
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    for call in (lambda: kernels.Mx4(codes, scales), lambda: kernels.Mx8(torch.zeros(4, 64, dtype=torch.float8_e4m3fn), scales),
+                 lambda: kernels.Mx4.empty(4, 64, "cpu"), lambda: kernels.gemm_mx4(torch.zeros(1, 64), codes, torch.zeros(1, 4)),
+                 lambda: kernels.mx8_pack(torch.zeros(4, 64), None)):
+        with pytest.raises(kernels.KernelError):
+            call()
+
+
+def test_a_launch_without_a_device_fails():
+    if torch.cuda.is_available():
+        pytest.skip("the operands are addresses of nothing: only where no kernel can be launched")
+    lib = kernels.library()
+    for rc, name in ((_gemm(lib), b"ta_gemm_mx4"), (_gemm(lib, glu=1, M=40), b"ta_gemm_mx4"), (_gemm8(lib), b"ta_gemm_mx4_mx8"),
+                     (_gemm8(lib, M=600, N=1024, K=2048), b"ta_gemm_mx4_mx8")):
+        assert rc != 0 and lib.ta_last_error().startswith(name), lib.ta_last_error()

@@ -1,0 +1,270 @@
+// To and from the blocks of mx.h: matrices to 4-bit weights and back, rows to 8 bits, and the two kernels that leave rows in
+// 8 bits where a step forms them: the norm behind the residual's addition, and the gated activation. All are bound by
+// memory: a lane takes 8 neighbouring values, the quad of its neighbours a block, so that the largest magnitude takes
+// two exchanges inside the quad.
+#include "mx.h"
+
+// ------------------------------------------------------------------ matrices
+// w [n][k] -> codes [n][k/2], scales [n][k/32]; a thread takes 8 values
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_pack_kernel(const T* __restrict__ w, long long ldw, uint8_t* __restrict__ codes,
+                                                       uint8_t* __restrict__ scales, long long n, int k) {
+  const long long pieces = k / 8, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const bool ok = at < n * pieces;               // a block's four threads are in or out together
+  const long long row = ok ? at / pieces : 0, p = ok ? at % pieces : 0;
+  float v[8];
+  mx_load8(w + row * ldw + p * 8, v);
+  const uint32_t byte = mx4_scale_byte(mx_top_quad(mx_top8(v)));
+  if (!ok) return;
+  uint32_t c = 0;
+  if (byte != MX_NAN) {
+    const float s = mx_inverse(byte);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c |= mx4_code(v[i] * s) << (4 * i);
+  }
+  *reinterpret_cast<uint32_t*>(codes + row * (k / 2) + p * 4) = c;
+  if (p % 4 == 0) scales[row * (k / 32) + p / 4] = (uint8_t)byte;
+}
+
+// the values that the codes stand for, exactly (bfloat16 holds them all but those below 2^-133 or above its range)
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_unpack_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                         T* __restrict__ out, long long ldo, long long n, int k) {
+  const long long pieces = k / 8, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= n * pieces) return;
+  const long long row = at / pieces, p = at % pieces;
+  const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + row * (k / 2) + p * 4);
+  const float s = mx_scale(scales[row * (k / 32) + p / 4]);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t m = c >> (4 * i) & 7u, sign = c >> (4 * i + 3) & 1u;
+    // exponent field 0: m / 2; else (1 + last bit / 2) 2^(field - 1)
+    const float a = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+    v[i] = (sign ? -a : a) * s;
+  }
+  T* o = out + row * ldo + p * 8;
+  if (sizeof(T) == 2) {
+    mx_u32x4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = f32x2_to_bf16x2_bits(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<mx_u32x4*>(o) = q;
+  } else {
+    reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+static bool mx_on(const void* p, int bytes) { return (uintptr_t)p % (uintptr_t)bytes == 0; }
+static int mx_blocks(const char* what, long long n, int k, int* grid) {
+  TA_REQUIRE(n >= 0 && k >= MX_BLOCK && k % MX_BLOCK == 0, "%s: %lld rows of %d: k goes by blocks of %d", what, n, k, MX_BLOCK);
+  const long long g = (n * (k / 8) + 255) / 256;
+  TA_REQUIRE(g <= 0x7fffffffLL, "%s: %lld rows of %d are more than a launch holds", what, n, k);
+  *grid = (int)g;
+  return 0;
+}
+
+// w [n][ldw] float32 or bfloat16, rows on 16 bytes.
+extern "C" int ta_mx4_pack(hipStream_t stream, int dtype, const void* w, long long ldw, void* codes, void* scales, long long n, int k) {
+  int grid;
+  TA_REQUIRE(dtype == TA_F32 || dtype == TA_BF16, "ta_mx4_pack: unknown dtype %d", dtype);
+  if (mx_blocks("ta_mx4_pack", n, k, &grid)) return 1;
+  TA_REQUIRE(ldw >= k && ldw * (dtype == TA_F32 ? 4 : 2) % 16 == 0 && mx_on(w, 16) && mx_on(codes, 16),
+             "ta_mx4_pack: rows %lld apart do not start on 16 bytes", ldw);
+  if (n == 0) return 0;
+  if (dtype == TA_F32)
+    mx4_pack_kernel<float><<<grid, 256, 0, stream>>>((const float*)w, ldw, (uint8_t*)codes, (uint8_t*)scales, n, k);
+  else
+    mx4_pack_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)w, ldw, (uint8_t*)codes, (uint8_t*)scales, n, k);
+  return ta_check_launch("ta_mx4_pack");
+}
+
+extern "C" int ta_mx4_unpack(hipStream_t stream, int dtype, const void* codes, const void* scales, void* out, long long ldo, long long n,
+                             int k) {
+  int grid;
+  TA_REQUIRE(dtype == TA_F32 || dtype == TA_BF16, "ta_mx4_unpack: unknown dtype %d", dtype);
+  if (mx_blocks("ta_mx4_unpack", n, k, &grid)) return 1;
+  TA_REQUIRE(ldo >= k && ldo * (dtype == TA_F32 ? 4 : 2) % 16 == 0 && mx_on(out, 16) && mx_on(codes, 16),
+             "ta_mx4_unpack: rows %lld apart do not start on 16 bytes", ldo);
+  if (n == 0) return 0;
+  if (dtype == TA_F32)
+    mx4_unpack_kernel<float><<<grid, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, (float*)out, ldo, n, k);
+  else
+    mx4_unpack_kernel<bf16_t><<<grid, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, (bf16_t*)out, ldo, n, k);
+  return ta_check_launch("ta_mx4_unpack");
+}
+
+// ------------------------------------------------------------------ rows
+template <typename T>
+__global__ __launch_bounds__(256) void mx8_pack_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes,
+                                                       uint8_t* __restrict__ scales, long long n, int k) {
+  const long long pieces = k / 8, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= n * pieces) return;                  // a block's four threads are in or out together
+  const long long row = at / pieces, p = at % pieces;
+  float v[8];
+  mx_load8(x + row * ldx + p * 8, v);
+  mx8_store(v, codes + row * k + p * 8, scales + row * (k / 32) + p / 4);
+}
+
+extern "C" int ta_mx8_pack(hipStream_t stream, int dtype, const void* x, long long ldx, void* codes, void* scales, long long n, int k) {
+  int grid;
+  TA_REQUIRE(dtype == TA_F32 || dtype == TA_BF16, "ta_mx8_pack: unknown dtype %d", dtype);
+  if (mx_blocks("ta_mx8_pack", n, k, &grid)) return 1;
+  TA_REQUIRE(ldx >= k && ldx * (dtype == TA_F32 ? 4 : 2) % 16 == 0 && mx_on(x, 16) && mx_on(codes, 16),
+             "ta_mx8_pack: rows %lld apart do not start on 16 bytes", ldx);
+  if (n == 0) return 0;
+  if (dtype == TA_F32)
+    mx8_pack_kernel<float><<<grid, 256, 0, stream>>>((const float*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, n, k);
+  else
+    mx8_pack_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, n, k);
+  return ta_check_launch("ta_mx8_pack");
+}
+
+// silu(gate) * up of [gate | up] rows, to 8 bits. The exponential and the quotient are the exact ones: a value next to a
+// rounding border of e4m3 then falls where 32-bit arithmetic puts it.
+template <typename T>
+__global__ __launch_bounds__(256) void swiglu_mx8_kernel(const T* __restrict__ gu, long long ld, const float* __restrict__ bias,
+                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, long long n, int d) {
+  const long long pieces = d / 8, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= n * pieces) return;
+  const long long row = at / pieces;
+  const int p = (int)(at % pieces);
+  float g[8], u[8];
+  mx_load8(gu + row * ld + p * 8, g);
+  mx_load8(gu + row * ld + d + p * 8, u);
+  if (bias) {
+    float bg[8], bu[8];
+    mx_load8(bias + p * 8, bg);
+    mx_load8(bias + d + p * 8, bu);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      g[i] += bg[i];
+      u[i] += bu[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
+  mx8_store(g, codes + row * d + p * 8, scales + row * (d / 32) + p / 4);
+}
+
+// gate_up [n][ld] float32 or bfloat16: d gates, then d ups; bias [2 d] or null.
+extern "C" int ta_swiglu_mx8(hipStream_t stream, int dtype, const void* gate_up, long long ld, const float* bias, void* codes, void* scales,
+                             long long n, int d) {
+  int grid;
+  TA_REQUIRE(dtype == TA_F32 || dtype == TA_BF16, "ta_swiglu_mx8: unknown dtype %d", dtype);
+  if (mx_blocks("ta_swiglu_mx8", n, d, &grid)) return 1;
+  TA_REQUIRE(ld >= 2LL * d && ld * (dtype == TA_F32 ? 4 : 2) % 16 == 0 && mx_on(gate_up, 16) && mx_on(codes, 16) && mx_on(bias, 16),
+             "ta_swiglu_mx8: rows %lld apart do not start on 16 bytes", ld);
+  if (n == 0) return 0;
+  if (dtype == TA_F32)
+    swiglu_mx8_kernel<float><<<grid, 256, 0, stream>>>((const float*)gate_up, ld, bias, (uint8_t*)codes, (uint8_t*)scales, n, d);
+  else
+    swiglu_mx8_kernel<bf16_t><<<grid, 256, 0, stream>>>((const bf16_t*)gate_up, ld, bias, (uint8_t*)codes, (uint8_t*)scales, n, d);
+  return ta_check_launch("ta_swiglu_mx8");
+}
+
+// ------------------------------------------------------------------ add + norm
+// v = x + delta (+ bias), stored to `stream` where there is one; y = v / sqrt(mean(v^2) + eps) * weight, to 8 bits. One
+// workgroup a row; HELD pieces of 8 values a thread stay in registers between the sum and the rows, 0: any number, read again
+// (by the thread that stored them).
+template <typename TD, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x, const TD* __restrict__ delta,
+                                                                  long long plane, int planes, const float* __restrict__ bias,
+                                                                  const float* __restrict__ weight, float eps, float* to,
+                                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int d) {
+  const size_t base = (size_t)blockIdx.x * d;
+  const int pieces = d / 8;
+  __shared__ float part[THREADS / 64];
+  float held[HELD ? HELD : 1][8];
+  float sum = 0.f;
+  const auto form = [&](int p, float* v) {
+    mx_load8(x + base + p * 8, v);
+    for (int j = 0; j < planes; ++j) {
+      float t[8];
+      mx_load8(delta + j * plane + base + p * 8, t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += t[i];
+    }
+    if (bias) {
+      float t[8];
+      mx_load8(bias + p * 8, t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += t[i];
+    }
+    if (to) {
+      reinterpret_cast<float4*>(to + base + p * 8)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(to + base + p * 8)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += v[i] * v[i];
+  };
+  if (HELD) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      const int p = threadIdx.x + h * THREADS;
+      if (p < pieces) form(p, held[h]);
+    }
+  } else {
+    for (int p = threadIdx.x; p < pieces; p += THREADS) form(p, held[0]);
+  }
+  sum = wave_sum(sum);
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = sum;
+  __syncthreads();
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) all += part[w];
+  const float r = rsqrtf(all / (float)d + eps);
+  const auto leave = [&](int p, const float* v) {
+    float w[8], y[8];
+    mx_load8(weight + p * 8, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[i] * r * w[i];
+    mx8_store(y, codes + base + p * 8, scales + base / 32 + p / 4);
+  };
+  if (HELD) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      const int p = threadIdx.x + h * THREADS;
+      if (p < pieces) leave(p, held[h]);
+    }
+  } else {
+    const float* from = to ? to : x;
+    for (int p = threadIdx.x; p < pieces; p += THREADS) {
+      float v[8];
+      mx_load8(from + base + p * 8, v);
+      leave(p, v);
+    }
+  }
+}
+
+template <typename TD>
+static void launch_norm(hipStream_t stream, const float* x, const TD* delta, int planes, const float* bias, const float* weight, float eps,
+                        float* to, uint8_t* codes, uint8_t* scales, int n, int d) {
+  const long long plane = (long long)n * d;
+#define MX_NORM(T, H) add_rmsnorm_mx8_kernel<TD, T, H><<<n, T, 0, stream>>>(x, delta, plane, planes, bias, weight, eps, to, codes, scales, d)
+  if (d <= 2048) MX_NORM(256, 1);
+  else if (d <= 4096) MX_NORM(512, 1);
+  else if (d <= 8192) MX_NORM(1024, 1);
+  else if (d <= 16384) MX_NORM(1024, 2);
+  else if (d <= 32768) MX_NORM(1024, 4);
+  else MX_NORM(1024, 0);
+#undef MX_NORM
+}
+
+// x [n][d] float32; delta: null (planes 0), or planes of [n][d], float32 or bfloat16, added in order; bias [d] or null; to: null, x,
+// or another [n][d] that gets the sum.
+extern "C" int ta_add_rmsnorm_mx8(hipStream_t stream, int delta_dtype, const float* x, const void* delta, int planes, const float* bias,
+                                  const float* weight, float eps, float* to, void* codes, void* scales, int n, int d) {
+  TA_REQUIRE(delta_dtype == TA_F32 || delta_dtype == TA_BF16, "ta_add_rmsnorm_mx8: unknown dtype %d", delta_dtype);
+  TA_REQUIRE(n >= 0 && d >= MX_BLOCK && d % MX_BLOCK == 0, "ta_add_rmsnorm_mx8: %d rows of %d: rows go by blocks of %d", n, d, MX_BLOCK);
+  TA_REQUIRE(planes >= 0 && planes <= TA_MAX_PLANES && (planes > 0) == (delta != nullptr), "ta_add_rmsnorm_mx8: %d planes", planes);
+  TA_REQUIRE(mx_on(x, 16) && mx_on(delta, 16) && mx_on(bias, 16) && mx_on(weight, 16) && mx_on(to, 16) && mx_on(codes, 16),
+             "ta_add_rmsnorm_mx8: rows do not start on 16 bytes");
+  TA_REQUIRE(to || (planes == 0 && !bias), "ta_add_rmsnorm_mx8: what is added goes nowhere");
+  if (n == 0) return 0;
+  if (delta_dtype == TA_F32)
+    launch_norm<float>(stream, x, (const float*)delta, planes, bias, weight, eps, to, (uint8_t*)codes, (uint8_t*)scales, n, d);
+  else
+    launch_norm<bf16_t>(stream, x, (const bf16_t*)delta, planes, bias, weight, eps, to, (uint8_t*)codes, (uint8_t*)scales, n, d);
+  return ta_check_launch("ta_add_rmsnorm_mx8");
+}

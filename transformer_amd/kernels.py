@@ -2868,3 +2868,233 @@ def memory_step(proj: torch.Tensor, offsets: Sequence[int], i_bias, f_bias, cap:
         _ptr(f_bias), c_float(cap), _ptr(state), _ptr(n_state), _ptr(m_state), _ptr(slots), c_int(B), c_int(H), c_int(dk),
         c_int(dv), c_float(q_scale), _ptr(norm_w), c_float(eps), _ptr(scratch), _ptr(out)))
     return out
+
+
+# ------------------------------------------------------------------ 4-bit weights, 8-bit rows
+# Blocks of 32 values along a row share a power of two 2^(b - 127), b a byte (255: the block is NaN). The scale of a block
+# is the smallest power of two with which its largest magnitude is at most the codes' largest value, 6 or 448.
+MX_BLOCK = 32
+_mx_types = {}
+
+
+def _mx(name: str, *types):
+    """The library's function with its argument types named once, so that a call hands over plain numbers: these launches are
+    as short as the Python in front of them."""
+    f = _mx_types.get(name)
+    if f is None:
+        f = getattr(library(), name)
+        f.argtypes, f.restype = types, c_int
+        _mx_types[name] = f
+    return f
+
+
+def _mx_stream():
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _here(what: str, *tensors):
+    """The launch goes to the current device's stream: every operand has to live there."""
+    at = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{at}")
+
+
+class Mx4:
+    """A matrix of 4-bit weights [n, k]: ``codes`` uint8 [n, k/2], two e2m1 values to a byte (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a
+    sign), the first in the low half; ``scales`` uint8 [n, k/32]. It stands where a weight tensor does."""
+    __slots__ = ("codes", "scales", "shape")
+    dtype = "mx4"                       # no torch.dtype: what asks for one finds another
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        _dev(codes, "codes", torch.uint8); _dev(scales, "scales", torch.uint8)
+        if codes.dim() != 2 or codes.shape[1] % 16 or codes.shape[1] < 16 or \
+                tuple(scales.shape) != (codes.shape[0], codes.shape[1] // 16):
+            raise KernelError(f"Mx4: codes {tuple(codes.shape)} / scales {tuple(scales.shape)}: rows go by blocks of {MX_BLOCK} "
+                              f"values, 16 bytes and one scale each")
+        if codes.data_ptr() % 16 or codes.get_device() != scales.get_device():
+            raise KernelError("Mx4: codes start on 16 bytes, beside their scales on one device")
+        self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], codes.shape[1] * 2)
+
+    @classmethod
+    def empty(cls, n: int, k: int, device) -> "Mx4":
+        if k % MX_BLOCK:
+            raise KernelError(f"Mx4: rows of {k} do not go by blocks of {MX_BLOCK}")
+        return cls(torch.empty(n, k // 2, dtype=torch.uint8, device=device),
+                   torch.empty(n, k // MX_BLOCK, dtype=torch.uint8, device=device))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+class Mx8:
+    """Rows of activations in 8 bits [m, k]: ``codes`` float8_e4m3fn [m, k], ``scales`` uint8 [m, k/32]."""
+    __slots__ = ("codes", "scales", "shape")
+    dtype = "mx8"
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        _dev(codes, "codes", torch.float8_e4m3fn); _dev(scales, "scales", torch.uint8)
+        if codes.dim() != 2 or codes.shape[1] % MX_BLOCK or codes.shape[1] < MX_BLOCK or \
+                tuple(scales.shape) != (codes.shape[0], codes.shape[1] // MX_BLOCK):
+            raise KernelError(f"Mx8: codes {tuple(codes.shape)} / scales {tuple(scales.shape)}: rows go by blocks of {MX_BLOCK} "
+                              f"values and one scale each")
+        if codes.data_ptr() % 16 or codes.get_device() != scales.get_device():
+            raise KernelError("Mx8: codes start on 16 bytes, beside their scales on one device")
+        self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], codes.shape[1])
+
+    @classmethod
+    def empty(cls, m: int, k: int, device) -> "Mx8":
+        if k % MX_BLOCK:
+            raise KernelError(f"Mx8: rows of {k} do not go by blocks of {MX_BLOCK}")
+        return cls(torch.empty(m, k, dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty(m, k // MX_BLOCK, dtype=torch.uint8, device=device))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def mx4_pack(w: torch.Tensor, out: Mx4) -> Mx4:
+    """w [n, k] float32 or bfloat16 to 4-bit weights, every value to the nearest (ties to the code with an even last bit). A
+    block that holds a NaN or an infinity becomes NaN."""
+    _dev(w, "w", contiguous=False)
+    n, ld = _rows2d(w, "w")
+    if tuple(w.shape) != out.shape:
+        raise KernelError(f"mx4_pack: w {tuple(w.shape)} out {out.shape}")
+    _here("mx4_pack", w, out.codes)
+    f = _mx("ta_mx4_pack", c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int)
+    _check(f(_mx_stream(), _code(w.dtype), w.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), n, w.shape[1]))
+    return out
+
+
+def mx4_unpack(w: Mx4, out: torch.Tensor) -> torch.Tensor:
+    """The values of the weights, out [n, k] float32 or bfloat16; both hold them exactly (short of the ends of bfloat16's range)."""
+    _dev(out, "out", contiguous=False)
+    n, ld = _rows2d(out, "out")
+    if tuple(out.shape) != w.shape:
+        raise KernelError(f"mx4_unpack: w {w.shape} out {tuple(out.shape)}")
+    _here("mx4_unpack", out, w.codes)
+    f = _mx("ta_mx4_unpack", c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int)
+    _check(f(_mx_stream(), _code(out.dtype), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ld, n, w.shape[1]))
+    return out
+
+
+def mx8_pack(x: torch.Tensor, out: Mx8) -> Mx8:
+    """x [m, k] float32 or bfloat16 to 8-bit rows, every value to the nearest, ties to even. A block that holds a NaN or an
+    infinity becomes NaN."""
+    _dev(x, "x", contiguous=False)
+    m, ld = _rows2d(x, "x")
+    if tuple(x.shape) != out.shape:
+        raise KernelError(f"mx8_pack: x {tuple(x.shape)} out {out.shape}")
+    _here("mx8_pack", x, out.codes)
+    f = _mx("ta_mx8_pack", c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int)
+    _check(f(_mx_stream(), _code(x.dtype), x.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), m, x.shape[1]))
+    return out
+
+
+def swiglu_mx8(gate_up: torch.Tensor, out: Mx8, bias: Optional[torch.Tensor] = None) -> Mx8:
+    """``swiglu`` in 32 bits with the result left as 8-bit rows: gate_up [m, 2*di] float32 or bfloat16, out [m, di]."""
+    _dev(gate_up, "gate_up", contiguous=False)
+    m, ld = _rows2d(gate_up, "gate_up")
+    d = out.shape[1]
+    if tuple(gate_up.shape) != (out.shape[0], 2 * d):
+        raise KernelError(f"swiglu_mx8: gate_up {tuple(gate_up.shape)} / out {out.shape}")
+    if bias is not None:
+        _dev(bias, "bias", torch.float32)
+        if bias.numel() != 2 * d:
+            raise KernelError("swiglu_mx8: bias must hold one entry per gate_up column")
+    _here("swiglu_mx8", gate_up, out.codes, bias)
+    f = _mx("ta_swiglu_mx8", c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_int)
+    _check(f(_mx_stream(), _code(gate_up.dtype), gate_up.data_ptr(), ld, None if bias is None else bias.data_ptr(),
+             out.codes.data_ptr(), out.scales.data_ptr(), m, d))
+    return out
+
+
+def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8, delta: Optional[torch.Tensor] = None,
+                    delta_bias: Optional[torch.Tensor] = None, stream: Optional[torch.Tensor] = None) -> Mx8:
+    """``add_rmsnorm`` with the normed rows left in 8 bits: v = x + delta + delta_bias goes back to x (to ``stream`` where one
+    is given, which then gets v also when nothing is added), rmsnorm(v) * weight to out. delta float32 or bfloat16 [m, d], or
+    [planes, m, d] whose planes are added in order."""
+    _dev(x, "x", torch.float32); _dev(weight, "weight", torch.float32)
+    m, d = out.shape
+    if tuple(x.shape) != (m, d) or weight.numel() != d:
+        raise KernelError(f"add_rmsnorm_mx8: x {tuple(x.shape)} weight {tuple(weight.shape)} out {out.shape}")
+    code, planes = F32, 0
+    if delta is not None:
+        _dev(delta, "delta")
+        if delta.shape[-2:] != x.shape or delta.dim() not in (2, 3):
+            raise KernelError(f"add_rmsnorm_mx8: delta is {tuple(delta.shape)}, x is {tuple(x.shape)}")
+        code, planes = _code(delta.dtype), 1 if delta.dim() == 2 else delta.shape[0]
+        if planes < 1:
+            raise KernelError("add_rmsnorm_mx8: delta has no planes")
+    if delta_bias is not None:
+        _dev(delta_bias, "delta_bias", torch.float32)
+        if delta_bias.numel() != d:
+            raise KernelError("add_rmsnorm_mx8: delta_bias must have one entry per column")
+    if stream is not None:
+        _dev(stream, "stream", torch.float32)
+        if stream.shape != x.shape:
+            raise KernelError(f"add_rmsnorm_mx8: stream is {tuple(stream.shape)}, x is {tuple(x.shape)}")
+    elif delta is not None or delta_bias is not None:
+        stream = x
+    _here("add_rmsnorm_mx8", x, weight, out.codes, delta, delta_bias, stream)
+    f = _mx("ta_add_rmsnorm_mx8", c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
+            c_int, c_int)
+    _check(f(_mx_stream(), code, x.data_ptr(), None if delta is None or m == 0 else delta.data_ptr(), planes if m else 0,
+             None if delta_bias is None else delta_bias.data_ptr(), weight.data_ptr(), eps,
+             None if stream is None else stream.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d))
+    return out
+
+
+MX4_MAX_ROWS = 64       # bfloat16 rows that ``gemm_mx4`` takes (ta_mx4_max_rows)
+
+
+def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, swiglu: bool = False) -> torch.Tensor:
+    """out = a @ w.T (+ bias) with 4-bit weights, sums in float32.
+
+    a bfloat16, at most ``MX4_MAX_ROWS`` rows (more: ``mx4_unpack`` and a product of many bfloat16 rows): the weights enter with
+    their exact values (one of 2^128 and more, which bfloat16 does not hold, as an infinity), out float32 or bfloat16. swiglu: w is [2*n, k] (gate rows, up rows) and out [m, n] = silu(a @ gate.T) *
+    (a @ up.T).
+
+    a ``Mx8``, any number of rows: the matrix cores multiply both as they are, and keep some 15 bits below the largest of
+    the 128 products that they add at a time; out bfloat16."""
+    if not isinstance(w, Mx4):
+        raise KernelError(f"gemm_mx4: the weights are an Mx4, not {type(w).__name__}")
+    n, k = w.shape
+    if isinstance(a, Mx8):
+        _dev(out, "out", torch.bfloat16, contiguous=False)
+        if swiglu:
+            raise KernelError("gemm_mx4: 8-bit rows leave gates and ups to swiglu_mx8")
+    else:
+        _dev(a, "a", torch.bfloat16, contiguous=False); _dev(out, "out", contiguous=False)
+        if swiglu and n % 2:
+            raise KernelError(f"gemm_mx4: {n} rows of weights are not gates and ups")
+    m = a.shape[0]
+    mo, ldo = _rows2d(out, "out")
+    cols = n // 2 if swiglu else n
+    if a.shape[1] != k or mo != m or out.shape[1] != cols:
+        raise KernelError(f"gemm_mx4: a {tuple(a.shape)} w {w.shape} out {tuple(out.shape)}")
+    if bias is not None:
+        _dev(bias, "bias", torch.float32)
+        if bias.numel() != n:
+            raise KernelError("gemm_mx4: bias must hold one entry per row of w")
+    if m == 0 or cols == 0:
+        return out
+    bp = None if bias is None else bias.data_ptr()
+    if isinstance(a, Mx8):
+        _here("gemm_mx4", a.codes, w.codes, out, bias)
+        f = _mx("ta_gemm_mx4_mx8", c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int)
+        _check(f(_mx_stream(), a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), bp, out.data_ptr(), ldo, m,
+                 cols, k))
+        return out
+    _here("gemm_mx4", a, w.codes, out, bias)
+    _, lda = _rows2d(a, "a")
+    f = _mx("ta_gemm_mx4", c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int,
+            c_int)
+    _check(f(_mx_stream(), _code(out.dtype), int(swiglu), a.data_ptr(), lda, w.codes.data_ptr(), w.scales.data_ptr(), bp, out.data_ptr(), ldo,
+             m, cols, k))
+    return out
