@@ -38,9 +38,22 @@ def open_model_source(path):
     return arch, cfg, file
 
 
-def load_model(path, dtype=None, device="cuda:0", verbose=False) -> DecoderModel:
+def _check_weights(weights, activations):
+    if weights not in (None, "mx4"):
+        raise ValueError(f"weights are kept as they are (None) or packed to \"mx4\", got {weights!r}")
+    if weights is None and activations not in (None, "bfloat16"):
+        raise ValueError(f"activations {activations!r} go with 4-bit weights")
+
+
+def load_model(path, dtype=None, device="cuda:0", verbose=False, weights=None, activations=None) -> DecoderModel:
     """dtype None: what the configuration's ``default_engine_dtype()`` says (config.json's
-    torch_dtype: float32 stays float32, everything else computes in bfloat16)."""
+    torch_dtype: float32 stays float32, everything else computes in bfloat16).
+
+    weights "mx4": the projections of the attention and of the feed-forward are packed to 4-bit weights with a scale
+    for every 32 (``kernels.Mx4``) once they are loaded; norms, embedding and output matrix stay as they are. A bfloat16
+    engine, and parts that take them (the Llama decoder's). activations "mx8": those products then read their rows in 8
+    bits as well, left so by the norms and the activation; None or "bfloat16": as they are."""
+    _check_weights(weights, activations)
     arch, cfg, file = open_model_source(path)
     if dtype is None:
         dtype = getattr(cfg, "default_engine_dtype", lambda: "bfloat16")()
@@ -57,6 +70,8 @@ def load_model(path, dtype=None, device="cuda:0", verbose=False) -> DecoderModel
 
     tensors = load_parameters(model.all_params(), arch.weight_sources(cfg, file.format), file,
                               model.dtype, model.device, where=str(path), progress=progress)
+    if weights == "mx4":
+        tensors = model.pack_mx4(tensors, activations)
     model.bind(tensors)
     file.close()
     import resource
@@ -74,11 +89,12 @@ def load_model(path, dtype=None, device="cuda:0", verbose=False) -> DecoderModel
 
 def random_model(config, seed: int = 0, dtype="bfloat16", device="cuda:0", std: float = 0.02,
                  norm_std: float = 0.1, architecture: str = "LlamaForCausalLM",
-                 num_layers=None) -> DecoderModel:
+                 num_layers=None, weights=None, activations=None) -> DecoderModel:
     """A model whose weights are drawn on the GPU (nothing touches the disk):
     matrices ~ N(0, std), norm weights 1 + N(0, norm_std), biases ~ N(0, std).
     ``num_layers`` builds only the first layers, for a configuration that offers
-    ``with_layers(n)``."""
+    ``with_layers(n)``. weights, activations: as in ``load_model``."""
+    _check_weights(weights, activations)
     import zlib
     from . import kernels
     from .weights.loader import storage_dtype
@@ -112,6 +128,8 @@ def random_model(config, seed: int = 0, dtype="bfloat16", device="cuda:0", std: 
             tensors[name] = t
     if tied:
         tensors["head.weight"] = tensors["embed.weight"]
+    if weights == "mx4":
+        tensors = model.pack_mx4(tensors, activations)
     model.bind(tensors)
     return model
 
@@ -120,7 +138,11 @@ def save_model(model: DecoderModel, folder, metadata=None):
     """Writes ``model`` (loaded, or drawn by ``random_model``) as a model folder: config.json
     and model.safetensors under the architecture's own tensor names, in the types the
     model holds them in. ``load_model(folder, same dtype)`` gives the same model back."""
+    from . import kernels
     from .weights.save import save_model_folder
+    packed = [n for n, t in model.tensors.items() if isinstance(t, kernels.Mx4)]
+    if packed:
+        raise ValueError(f"a model with 4-bit weights is not written: {len(packed)} matrices are packed (first: {packed[0]})")
     arch, cfg = model.architecture, model.config
     if cfg.tie_embeddings is None and model.w["embed"].data_ptr() == model.w["head"].data_ptr():
         import dataclasses

@@ -67,6 +67,8 @@ class Inference:
     timers: bool = False        # GPU time per kind of part (steps then run eagerly)
     random: Optional[str] = None   # instead of ``model``: a config.json or a shape name; weights from ``seed``
     layers: Optional[int] = None
+    weights: Optional[str] = None       # "mx4": 4-bit weights
+    activations: Optional[str] = None   # "mx8": and rows in 8 bits
 
     @classmethod
     def load(cls) -> Optional["Inference"]:
@@ -121,10 +123,11 @@ def infer(inf: Inference, stream=sys.stdout):
         d = dict(SHAPES[inf.random][1]) if inf.random in SHAPES else json.loads(Path(inf.random).read_text())
         arch = architecture_of_config_json(d)
         model = random_model(arch.config_from_dict(d), inf.seed, inf.dtype or "bfloat16", device,
-                             architecture=arch.name, num_layers=inf.layers)
+                             architecture=arch.name, num_layers=inf.layers, weights=inf.weights,
+                             activations=inf.activations)
         where = Path(inf.random).parent if inf.random not in SHAPES else Path(".")
     else:
-        model = load_model(inf.model, inf.dtype, device, verbose=True)
+        model = load_model(inf.model, inf.dtype, device, verbose=True, weights=inf.weights, activations=inf.activations)
         where = inf.model
     prompts = [prompt_to_tokens(p, where) for p in inf.prompt]
     # MAX_STEPS counts calls of the model; every call yields one token
@@ -172,6 +175,10 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
     g.add_argument("--dtype", choices=["bfloat16", "float32"], default=None,
                    help="the engine's type; default: what config.json's torch_dtype says (float32 stays "
                         "float32, everything else computes in bfloat16)")
+    g.add_argument("--weights", choices=["mx4"], default=None,
+                   help="mx4: pack the projections to 4-bit weights with a scale for every 32")
+    g.add_argument("--activations", choices=["bfloat16", "mx8"], default=None,
+                   help="with --weights mx4: what those products read their rows in")
     g.add_argument("--backend", choices=["hip", "ref"], default="hip",
                    help="ref: the plain float32 kernels of the device (sums in 32 bits in an order that does "
                         "not depend on the batch), whatever --dtype says; the "
@@ -208,7 +215,8 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
                             as_user=a.as_user, temperature=a.temperature, top_p=a.top_p,
                             top_k=a.top_k, max_steps=a.max_steps,
                             dtype="float32" if a.backend == "ref" else a.dtype, seed=a.seed,
-                            timers=a.timers, random=a.random, layers=a.layers)
+                            timers=a.timers, random=a.random, layers=a.layers, weights=a.weights,
+                            activations=a.activations)
             infer(inf)
             return 0
         if not a.model:
@@ -219,7 +227,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
                         as_user=a.as_user, temperature=a.temperature, top_p=a.top_p,
                         top_k=a.top_k, max_steps=a.max_steps,
                         dtype="float32" if a.backend == "ref" else a.dtype, seed=a.seed,
-                        timers=a.timers)
+                        timers=a.timers, weights=a.weights, activations=a.activations)
         infer(inf)
         return 0
     if a.cmd == "random":

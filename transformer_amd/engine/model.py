@@ -129,6 +129,39 @@ class DecoderModel:
         out["head.weight"] = Param((s.vocab, s.hidden), "matrix")
         return out
 
+    def all_mx4(self) -> List[str]:
+        """The matrices that parts of this model also take with 4-bit weights."""
+        return [n for i, b in enumerate(self.blocks) if hasattr(b, "all_mx4") for n in b.all_mx4(f"blocks.{i}.")]
+
+    def pack_mx4(self, tensors: Dict[str, torch.Tensor], activations=None) -> Dict[str, torch.Tensor]:
+        """``tensors`` with every matrix of ``all_mx4`` packed to 4-bit weights; the others in storage of their own, so that
+        nothing keeps the wide matrices. activations: "bfloat16" (also None) or "mx8", what the products read their rows in."""
+        if activations not in (None, "bfloat16", "mx8"):
+            raise ValueError(f"activations are \"bfloat16\" or \"mx8\", got {activations!r}")
+        if self.dtype != torch.bfloat16:
+            raise ValueError("4-bit weights belong to an engine that computes in bfloat16")
+        names = set(self.all_mx4())
+        odd = sorted(n for n in names if tensors[n].shape[1] % kernels.MX_BLOCK)
+        if not names or odd:
+            raise ValueError("no part of this model takes 4-bit weights" if not names else
+                             f"4-bit weights go by blocks of {kernels.MX_BLOCK} along a row: {odd[0]} is {tuple(tensors[odd[0]].shape)}")
+        if activations == "mx8" and not all(getattr(b, "takes_rows8", False) for b in self.blocks):
+            raise ValueError("rows in 8 bits need blocks of the plain pre-norm arrangement")
+        out, own = {}, {}
+        with torch.cuda.device(self.device):
+            for n, t in tensors.items():
+                if n in names:
+                    out[n] = kernels.mx4_pack(t, kernels.Mx4.empty(t.shape[0], t.shape[1], self.device))
+                else:                       # a shared table stays shared
+                    key = (t.data_ptr(), tuple(t.shape), t.dtype)
+                    if key not in own:
+                        own[key] = t.clone()
+                    out[n] = own[key]
+        if activations == "mx8":
+            for b in self.blocks:
+                b.read_rows8(True)
+        return out
+
     def bind(self, tensors: Dict[str, torch.Tensor]) -> None:
         want = self.all_params()
         missing = sorted(set(want) - set(tensors))
@@ -158,7 +191,11 @@ class DecoderModel:
         def visit(part):
             nonlocal total
             for t in getattr(part, "w", {}).values():
-                if t.data_ptr() not in seen:
+                if isinstance(t, kernels.Mx4):
+                    if t.codes.data_ptr() not in seen:
+                        seen.add(t.codes.data_ptr())
+                        total += t.nbytes()
+                elif t.data_ptr() not in seen:
                     seen.add(t.data_ptr())
                     total += t.numel() * t.element_size()
             for c in part.children().values():

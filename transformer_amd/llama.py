@@ -20,13 +20,13 @@ class Llama:
         self._cache = None
 
     @classmethod
-    def from_pretrained(cls, path, dtype="bfloat16", device="cuda:0", **kw) -> "Llama":
-        """path: a folder with config.json and safetensors, or a .gguf file."""
-        return cls(load_model(path, dtype, device), **kw)
+    def from_pretrained(cls, path, dtype="bfloat16", device="cuda:0", weights=None, activations=None, **kw) -> "Llama":
+        """path: a folder with config.json and safetensors, or a .gguf file. weights, activations: as in ``load_model``."""
+        return cls(load_model(path, dtype, device, weights=weights, activations=activations), **kw)
 
     @classmethod
-    def random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", **kw) -> "Llama":
-        return cls(random_model(config, seed, dtype, device), **kw)
+    def random(cls, config, seed: int = 0, dtype="bfloat16", device="cuda:0", weights=None, activations=None, **kw) -> "Llama":
+        return cls(random_model(config, seed, dtype, device, weights=weights, activations=activations), **kw)
 
     @property
     def cache(self):

@@ -20,7 +20,7 @@ from .. import kernels
 from ..cache.storage import KVNeed
 from ..weights.loader import Param
 from .base import Part, PartError, build_part, register_part
-from .linear import adds_in_place, aligned_rows, finish, linear, linear_delta
+from .linear import adds_in_place, aligned_rows, finish, linear, linear_delta, rows8
 
 
 @dataclass(frozen=True)
@@ -45,6 +45,8 @@ class KeyUnitPlanner:
 
 
 class CachedAttention(Part):
+    mx4_weights = ("qkv.weight", "out.weight")
+
     @property
     def graph_safe(self) -> bool:
         return bool(getattr(self.position, "graph_safe", False))
@@ -95,6 +97,8 @@ class CachedAttention(Part):
         return adds_in_place(nt, self.w["out.weight"], self.dtype)
 
     def _out(self, o, ctx, fold, into):
+        if self.rows8:
+            o = rows8(o, ctx.ws, "attention.o8")
         if fold is not None:
             kernels.gemm_skinny(o, self.w["out.weight"], None, bias=self.w.get("out.bias"), fold=fold)
             return None
@@ -107,8 +111,10 @@ class CachedAttention(Part):
         residual stream that the output projection has then added itself to. ``norm`` stands for h."""
         nt = h.shape[0]
         width = (self.nq + 2 * self.nkv) * self.dh
+        if self.rows8:
+            h = rows8(h, ctx.ws, "block.h8")
         qkv = linear(h, self.w["qkv.weight"], ctx.ws.take("attention.qkv", (nt, width), self.dtype),
-                     scale=scale, norm=norm)
+                     scale=scale, norm=norm, ws=ctx.ws)
         kc, vc, group = cache.layer_kv(layer)
         meta = ctx.kv[group]
         o = ctx.ws.take("attention.o", (nt, self.nq * self.dh), self.dtype)

@@ -104,6 +104,10 @@ def build_part(spec, dtype: torch.dtype, device):
 
 class Part:
     """Base class: parameter declaration and binding."""
+    # matrices that the part also takes as ``kernels.Mx4`` (``load_model(weights="mx4")``), and whether its products then read
+    # their rows in 8 bits
+    mx4_weights = ()
+    rows8 = False
 
     def params(self) -> Dict[str, Param]:
         return {}
@@ -127,6 +131,19 @@ class Part:
         for cname, child in self.children().items():
             out.update(child.all_params(prefix + cname + "."))
         return out
+
+    def all_mx4(self, prefix: str = ""):
+        """Names, as ``all_params`` has them, of the matrices that may have 4-bit weights."""
+        names = [prefix + n for n in self.mx4_weights]
+        for cname, child in self.children().items():
+            names += child.all_mx4(prefix + cname + ".")
+        return names
+
+    def read_rows8(self, on: bool) -> None:
+        if self.mx4_weights:
+            self.rows8 = on
+        for child in self.children().values():
+            child.read_rows8(on)
 
     def bind_all(self, tensors: Dict[str, torch.Tensor], prefix: str = "") -> None:
         self.bind({n: tensors[prefix + n] for n in self.params()})

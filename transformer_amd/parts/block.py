@@ -13,9 +13,13 @@ import torch
 
 from .. import kernels
 from .base import Part, build_part, register_part, span
+from .linear import empty8
+from .norm import RMSNorm
 
 
 class PreNormBlock(Part):
+    takes_rows8 = True      # the norms can leave their rows in 8 bits for parts that read them so
+
     def __init__(self, spec, dtype, device):
         self.dtype = dtype
         self.norm1 = build_part(spec.norm1, dtype, device)
@@ -62,6 +66,13 @@ class PreNormBlock(Part):
         f = getattr(part, what, None)
         return f is not None and bool(f(nt))
 
+    @staticmethod
+    def _rows_for(part, norm, h, ctx):
+        """Where the norm in front of a part leaves its rows: in 8 bits where the part's products read them so."""
+        if getattr(part, "rows8", False) and isinstance(norm, RMSNorm):
+            return empty8(h.shape, ctx.ws, "block.h8")
+        return h
+
     def _normed(self, norm, part, pending, x):
         """The norm for a float32 part whose first product goes over it itself; None where its own kernel runs."""
         if self.dtype == torch.float32 and isinstance(pending, tuple) and pending[0] is None and pending[1] is None \
@@ -103,7 +114,7 @@ class PreNormBlock(Part):
         served, or "normed" (it has left norm1's rows in the shared buffer). after: the block that
         runs next, if any. Returns the new pending."""
         nt = x.shape[0]
-        h = ctx.ws.take("block.h", x.shape, self.dtype)
+        h = rows = ctx.ws.take("block.h", x.shape, self.dtype)
         kw = {}
         if isinstance(pending, kernels.RowScale):
             kw["scale"] = pending                  # h already holds the rows, not yet scaled
@@ -111,15 +122,16 @@ class PreNormBlock(Part):
             kw["norm"] = self._normed(self.norm1, self.mixer, pending, x)
             if kw["norm"] is None:
                 del kw["norm"]
+                rows = self._rows_for(self.mixer, self.norm1, h, ctx)
                 with span(ctx, "norm"):
-                    self.norm1.run(x, h, pending[0], pending[1])
+                    self.norm1.run(x, rows, pending[0], pending[1])
         # the rows that the side part reads: the stream itself where the engine computes in float32
         xcast = None
         if self.side is not None:
             xcast = x if self.dtype == torch.float32 else ctx.ws.take("block.xcast", x.shape, self.dtype)
         if self.ffn is None:
             with span(ctx, "mixer"):
-                pending = self.mixer.run(h, ctx, cache, layer, writes_cache, **kw)
+                pending = self.mixer.run(rows, ctx, cache, layer, writes_cache, **kw)
             if self.side is None:
                 return pending
             with span(ctx, "norm"):
@@ -134,7 +146,8 @@ class PreNormBlock(Part):
         if "fold" not in kw and self._offers(self.mixer, "can_add", nt):
             kw["into"] = x
         with span(ctx, "mixer"):
-            pending = self.mixer.run(h, ctx, cache, layer, writes_cache, **kw)
+            pending = self.mixer.run(rows, ctx, cache, layer, writes_cache, **kw)
+        rows = h
         kw2 = {}
         if "fold" in kw:
             kw2["scale"] = kw["fold"].scale()
@@ -142,17 +155,18 @@ class PreNormBlock(Part):
             kw2["norm"] = self._normed(self.norm2, self.ffn, pending, x)
             if kw2["norm"] is None:
                 del kw2["norm"]
+                rows = self._rows_for(self.ffn, self.norm2, h, ctx)
                 with span(ctx, "norm"):
-                    self.norm2.run(x, h, pending[0], pending[1])
+                    self.norm2.run(x, rows, pending[0], pending[1])
         if self.side is not None:
             if fusable and self._offers(self.ffn, "can_fold", nt):
                 with span(ctx, "ffn"):
-                    self.ffn.run(h, ctx, fold=self._cast_fold(x, xcast, ctx), **kw2)
+                    self.ffn.run(rows, ctx, fold=self._cast_fold(x, xcast, ctx), **kw2)
             else:
                 if self._offers(self.ffn, "can_add", nt):
                     kw2["into"] = x
                 with span(ctx, "ffn"):
-                    pending = self.ffn.run(h, ctx, **kw2)
+                    pending = self.ffn.run(rows, ctx, **kw2)
                 with span(ctx, "norm"):
                     kernels.stream_add(x, pending[0], pending[1], None if xcast is x else xcast)
             return self._run_side(x, xcast, ctx, after, h)
@@ -162,14 +176,14 @@ class PreNormBlock(Part):
             handover = entry(x, ctx) if entry is not None else None
         if handover is not None:
             with span(ctx, "ffn"):
-                self.ffn.run(h, ctx, fold=handover, **kw2)
+                self.ffn.run(rows, ctx, fold=handover, **kw2)
             return handover.scale()
         # Where rows of the model's own may join the stream before anything reads it (no ``after``), float32 leaves the
         # add to the norm behind them: how many rows a step has would otherwise decide which of the two comes first
         if (after is not None or self.dtype != torch.float32) and self._offers(self.ffn, "can_add", nt):
             kw2["into"] = x
         with span(ctx, "ffn"):
-            return self.ffn.run(h, ctx, **kw2)
+            return self.ffn.run(rows, ctx, **kw2)
 
 
 register_part("prenorm", PreNormBlock)

@@ -12,12 +12,13 @@ import torch
 from .. import kernels
 from ..weights.loader import Param
 from .base import Part, PartError, register_part
-from .linear import activated, adds_in_place, linear, linear_delta
+from .linear import activated, adds_in_place, empty8, linear, linear_delta, of_rows, rows8
 
 
 class SwiGLU(Part):
     graph_safe = True
     limits = None           # (limit, slope, shift) of the limited activation; None: silu(gate) * up
+    mx4_weights = ("gate_up.weight", "down.weight")
 
     def __init__(self, spec, dtype, device):
         self.spec, self.dtype = spec, dtype
@@ -49,29 +50,39 @@ class SwiGLU(Part):
         residual stream that the down projection has then added itself to. ``scale``: the rows
         of h still lack their norm's factor; ``norm`` (float32) stands for h."""
         s, nt = self.spec, h.shape[0]
+        if self.rows8:
+            # 8-bit rows: the product leaves gates and ups, the activation's kernel the down product's rows
+            gu = linear(rows8(h, ctx.ws, "block.h8"), self.w["gate_up.weight"],
+                        ctx.ws.take("swiglu.gate_up", (nt, 2 * s.intermediate), self.dtype))
+            act8 = kernels.swiglu_mx8(gu, empty8((nt, s.intermediate), ctx.ws, "swiglu.act8"), self.w.get("gate_up.bias"))
+            return linear_delta(act8, self.w["down.weight"], ctx.ws, "swiglu.delta"), self.w.get("down.bias")
         act = ctx.ws.take("swiglu.act", (nt, s.intermediate), self.dtype)
+        gate_up = of_rows(nt, self.w["gate_up.weight"], ctx.ws)
         if norm is not None:
-            kernels.gemm_normed(norm, self.w["gate_up.weight"], act, self.w.get("gate_up.bias"), glu=True)
-        elif scale is not None or kernels.skinny_wins(h, self.w["gate_up.weight"]):
+            kernels.gemm_normed(norm, gate_up, act, self.w.get("gate_up.bias"), glu=True)
+        elif isinstance(gate_up, kernels.Mx4):
+            # few rows against 4-bit weights: the product applies the activation itself
+            kernels.gemm_mx4(h, gate_up, act, self.w.get("gate_up.bias"), swiglu=True)
+        elif scale is not None or kernels.skinny_wins(h, gate_up):
             # few rows: the product applies the activation itself and [nt, 2*di] is never stored
-            kernels.gemm_skinny(h, self.w["gate_up.weight"], act, swiglu=True,
+            kernels.gemm_skinny(h, gate_up, act, swiglu=True,
                                 bias=self.w.get("gate_up.bias"), scale=scale, limits=self.limits)
-        elif h.dtype == torch.bfloat16 and kernels.mid_takes(nt, self.w["gate_up.weight"]):
+        elif h.dtype == torch.bfloat16 and kernels.mid_takes(nt, gate_up):
             # up to 64 rows the product of our own applies the activation itself: 44 to 54 us on
             # the 8B shape where the vendor library's product and the activation's kernel take 55
-            kernels.gemm_mid(h, self.w["gate_up.weight"], act, swiglu=True, bias=self.w.get("gate_up.bias"),
+            kernels.gemm_mid(h, gate_up, act, swiglu=True, bias=self.w.get("gate_up.bias"),
                              limits=self.limits)
-        elif self.limits is None and kernels.simple_glu_takes(h, self.w["gate_up.weight"]):
+        elif self.limits is None and kernels.simple_glu_takes(h, gate_up):
             # few float32 rows: the product applies the activation itself, with the same bits
-            kernels.gemm_simple_glu(h, self.w["gate_up.weight"], act, self.w.get("gate_up.bias"))
-        elif self.limits is None and kernels.split_glu_takes(h, self.w["gate_up.weight"]):
+            kernels.gemm_simple_glu(h, gate_up, act, self.w.get("gate_up.bias"))
+        elif self.limits is None and kernels.split_glu_takes(h, gate_up):
             # and many
-            kernels.gemm_split_glu(h, self.w["gate_up.weight"], act, self.w.get("gate_up.bias"))
-        elif kernels.glu_pays(h, self.w["gate_up.weight"]):
+            kernels.gemm_split_glu(h, gate_up, act, self.w.get("gate_up.bias"))
+        elif kernels.glu_pays(h, gate_up):
             # many bfloat16 rows: likewise, gates and ups joined before they are rounded
-            kernels.gemm_glu(h, self.w["gate_up.weight"], act, bias=self.w.get("gate_up.bias"), limits=self.limits)
+            kernels.gemm_glu(h, gate_up, act, bias=self.w.get("gate_up.bias"), limits=self.limits)
         else:
-            gu = linear(h, self.w["gate_up.weight"],
+            gu = linear(h, gate_up,
                         ctx.ws.take("swiglu.gate_up", (nt, 2 * s.intermediate), self.dtype))
             if self.limits is None:
                 kernels.swiglu(gu, act, self.w.get("gate_up.bias"))
@@ -88,6 +99,7 @@ class GLU(SwiGLU):
     """The same feed-forward with the activation as a parameter of the spec ("silu", "gelu_tanh",
     "limited"). Silu and the limited form take every path of ``SwiGLU`` (the products that apply it
     themselves included); another activation runs the product and then the activation's kernel."""
+    mx4_weights = ()
 
     def __init__(self, spec, dtype, device):
         super().__init__(spec, dtype, device)

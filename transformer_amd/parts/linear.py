@@ -47,10 +47,33 @@ class Workspace:
         self.take(name, (numel,), dtype)
 
 
+def of_rows(rows: int, weight, ws: Optional[Workspace]):
+    """The matrix that a product of so many bfloat16 rows reads: 4-bit weights as they are for few rows, for more their exact
+    values in bfloat16, laid out again for every product in scratch that all of them share."""
+    if not isinstance(weight, kernels.Mx4) or rows <= kernels.MX4_MAX_ROWS:
+        return weight
+    if ws is None:
+        wide = torch.empty(weight.shape, dtype=torch.bfloat16, device=weight.device)
+    else:
+        wide = ws.take("mx4.wide", weight.shape, torch.bfloat16)
+    return kernels.mx4_unpack(weight, wide)
+
+
+def rows8(x, ws: Workspace, name: str) -> "kernels.Mx8":
+    """x in 8 bits; as it is where it has come so."""
+    return x if isinstance(x, kernels.Mx8) else kernels.mx8_pack(x, empty8(x.shape, ws, name))
+
+
+def empty8(shape, ws: Workspace, name: str) -> "kernels.Mx8":
+    return kernels.Mx8(ws.take(name, shape, torch.float8_e4m3fn),
+                       ws.take(name + ".scales", (shape[0], shape[1] // kernels.MX_BLOCK), torch.uint8))
+
+
 def linear(x: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor], scale=None,
-           fold=None, norm=None) -> torch.Tensor:
+           fold=None, norm=None, ws: Optional[Workspace] = None) -> torch.Tensor:
     """out[nt, n] = x[nt, k] @ weight[n, k]^T. x and weight share a dtype, or the weight is
-    a float32 matrix of a bfloat16 engine (its file stores it in 32 bits and it stays so).
+    a float32 matrix of a bfloat16 engine (its file stores it in 32 bits and it stays so), or
+    it is a ``kernels.Mx4`` (ws: where its values are laid out for many bfloat16 rows).
 
     scale (``kernels.RowScale``): the rows of x still lack their norm's factor, which the
     product applies. fold (``kernels.NormFold``): the product is added to the residual stream
@@ -61,6 +84,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor], s
         return kernels.gemm_normed(norm, weight, out)
     if scale is not None or fold is not None:
         return kernels.gemm_skinny(x, weight, out, scale=scale, fold=fold)
+    if isinstance(weight, kernels.Mx4):
+        if isinstance(x, kernels.Mx8) or x.shape[0] <= kernels.MX4_MAX_ROWS:
+            return kernels.gemm_mx4(x, weight, out)
+        weight = of_rows(x.shape[0], weight, ws)
     mixed = x.dtype == torch.bfloat16 and weight.dtype == torch.float32
     if x.dtype != weight.dtype and not mixed:
         raise kernels.KernelError(f"linear: activations are {x.dtype}, weights {weight.dtype}")
@@ -164,6 +191,9 @@ def linear_delta(x: torch.Tensor, weight: torch.Tensor, ws: Workspace, name: str
     is, and nothing is returned; a prompt's norm then reads the stream alone instead of reading
     stream and delta and writing the stream back (2,048 tokens of the 8B shape: 21 to 10 us)."""
     nt, n = x.shape[0], weight.shape[0]
+    if isinstance(x, kernels.Mx8):                 # the 8-bit product rounds to bfloat16
+        return kernels.gemm_mx4(x, weight, ws.take(name, (nt, n), torch.bfloat16))
+    weight = of_rows(nt, weight, ws)
     if into is not None:
         if not adds_in_place(nt, weight, x.dtype) or into.shape != (nt, n) or into.dtype != torch.float32:
             raise kernels.KernelError(f"linear_delta: cannot add {tuple(x.shape)} x {tuple(weight.shape)} "

@@ -30,8 +30,12 @@ class RMSNorm(Part):
     def run(self, x: torch.Tensor, out: torch.Tensor, delta: Optional[torch.Tensor] = None,
             delta_bias: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None, shift=None):
         """x: float32 [nt, size], updated in place by the pending delta unless
-        ``rows`` selects the rows to normalise. out: engine dtype. ``delta`` may be a
+        ``rows`` selects the rows to normalise. out: engine dtype, or ``kernels.Mx8``. ``delta`` may be a
         ``kernels.GatedDelta`` (what a gated sublayer leaves to be added)."""
+        if isinstance(out, kernels.Mx8):
+            if shift is not None or rows is not None or isinstance(delta, kernels.GatedDelta):
+                raise ValueError("rows in 8 bits are normed whole, behind a plain delta")
+            return kernels.add_rmsnorm_mx8(x, self.gain(), self.eps, out, delta, delta_bias)
         if shift is not None:
             # a single-token step's token shift rides on the norm (``kernels.gated_add_rmsnorm``)
             if delta is not None and not isinstance(delta, kernels.GatedDelta):
