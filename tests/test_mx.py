@@ -13,8 +13,9 @@ def _gemm(lib, M=4, N=64, K=64, x=AT, codes=AT, ldx=None, ldo=None, dtype=1, glu
                            c_longlong(N if ldo is None else ldo), c_int(M), c_int(N), c_int(K))
 
 
-def _gemm8(lib, M=4, N=64, K=64, x=AT, ldo=None):
-    return lib.ta_gemm_mx4_mx8(None, x, AT, AT, AT, None, AT, c_longlong(N if ldo is None else ldo), c_int(M), c_int(N), c_int(K))
+def _gemm8(lib, M=4, N=64, K=64, x=AT, ldo=None, xs=AT, scratch=None, room=0):
+    return lib.ta_gemm_mx4_mx8(None, x, xs, AT, AT, None, AT, c_longlong(N if ldo is None else ldo), c_int(M), c_int(N), c_int(K), scratch,
+                               c_longlong(room))
 
 
 def _refused(rc, name):
@@ -26,11 +27,16 @@ def test_products_refuse_what_their_kernels_do_not_take():
     lib = kernels.library()
     off = c_void_p((1 << 20) + 8)
     for kw in (dict(K=48), dict(K=0), dict(M=-1), dict(N=0), dict(x=off), dict(codes=off), dict(ldx=68), dict(ldx=32), dict(ldo=63), dict(dtype=2),
-               dict(M=65), dict(N=1 << 30, glu=1)):
+               dict(M=65), dict(N=1 << 30, glu=1), dict(ldx=(1 << 24) + 8), dict(K=(1 << 24) + 32)):
         _refused(_gemm(lib, **kw), b"ta_gemm_mx4:")
-    for kw in (dict(K=48), dict(M=-1), dict(N=0), dict(x=off), dict(ldo=63), dict(M=2147483647, N=2147483647)):
+    for kw in (dict(K=48), dict(M=-1), dict(N=0), dict(x=off), dict(ldo=63), dict(M=2147483647, N=2147483647), dict(K=(1 << 23) + 32),
+               dict(M=65, K=96), dict(M=65, K=96, scratch=AT, room=(65 + 64) * 16 - 1), dict(M=65, K=96, scratch=c_void_p((1 << 20) + 8), room=1 << 20),
+               dict(M=65, K=512, xs=c_void_p((1 << 20) + 1))):
         _refused(_gemm8(lib, **kw), b"ta_gemm_mx4_mx8:")
     assert lib.ta_mx4_max_rows() == kernels.MX4_MAX_ROWS
+    lib.ta_gemm_mx4_mx8_scratch.restype = c_longlong
+    for M, N, K, need in ((kernels.MX8_FEW_ROWS, 70, 96, 0), (kernels.MX8_FEW_ROWS + 1, 70, 96, 135 * 16), (65, 70, 512, 0), (65, 70, 544, 135 * 32)):
+        assert lib.ta_gemm_mx4_mx8_scratch(c_int(M), c_int(N), c_int(K)) == need
     assert _gemm(lib, M=0) == 0 and _gemm8(lib, M=0) == 0
 
 

@@ -229,7 +229,9 @@ def test_products_of_8_bit_rows(m, n, k):
         _close(got, U.values8(x.codes, x.scales), U.values4(w.codes, w.scales), ALIGNED, False, bias)
 
 
-@pytest.mark.parametrize("m,n,k", [(1021, 1376, 2080), (600, 4100, 448), (2011, 260, 1056), (4400, 144, 64)])
+# tiles of every size: their rule goes by how many there are
+@pytest.mark.parametrize("m,n,k", [(1021, 1376, 2080), (600, 4100, 448), (2011, 260, 1056), (4400, 144, 64), (2050, 2100, 224), (2049, 2056, 640),
+                                   (4100, 4103, 160), (4097, 4104, 512), (513, 8200, 96)])
 def test_products_of_many_8_bit_rows(m, n, k):
     w, x = _weights(n, k, 3), _rows8(m, k, 3)
     got = kernels.gemm_mx4(x, w, torch.empty(m, n, device=DEV, dtype=torch.bfloat16))

@@ -3051,6 +3051,7 @@ def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8,
 
 
 MX4_MAX_ROWS = 64       # bfloat16 rows that ``gemm_mx4`` takes (ta_mx4_max_rows)
+MX8_FEW_ROWS = 64       # 8-bit rows up to which it goes without scratch (MX_FEW_ROWS8 of csrc/mx_gemm.hip)
 
 
 def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, swiglu: bool = False) -> torch.Tensor:
@@ -3087,9 +3088,15 @@ def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, 
     bp = None if bias is None else bias.data_ptr()
     if isinstance(a, Mx8):
         _here("gemm_mx4", a.codes, w.codes, out, bias)
-        f = _mx("ta_gemm_mx4_mx8", c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int)
-        _check(f(_mx_stream(), a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), bp, out.data_ptr(), ldo, m,
-                 cols, k))
+        f = _mx("ta_gemm_mx4_mx8", c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int,
+                c_void_p, c_longlong)
+        xs, ws = a.scales.data_ptr(), w.scales.data_ptr()
+        scratch, need = None, 0
+        if m > MX8_FEW_ROWS and (k % 512 or (xs | ws) % 16):    # scales whose rows are off 16 bytes are laid out again
+            need = (m + n) * (-(-k // 512) * 16)
+            scratch = torch.empty(need, dtype=torch.uint8, device=out.device)
+        _check(f(_mx_stream(), a.codes.data_ptr(), xs, w.codes.data_ptr(), ws, bp, out.data_ptr(), ldo, m, cols, k,
+                 None if scratch is None else scratch.data_ptr(), need))
         return out
     _here("gemm_mx4", a, w.codes, out, bias)
     _, lda = _rows2d(a, "a")
