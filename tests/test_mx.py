@@ -8,9 +8,9 @@ from transformer_amd import kernels
 AT = c_void_p(1 << 20)
 
 
-def _gemm(lib, M=4, N=64, K=64, x=AT, codes=AT, ldx=None, ldo=None, dtype=1, glu=0):
+def _gemm(lib, M=4, N=64, K=64, x=AT, codes=AT, ldx=None, ldo=None, dtype=1, glu=0, scratch=None, room=0):
     return lib.ta_gemm_mx4(None, c_int(dtype), c_int(glu), x, c_longlong(K if ldx is None else ldx), codes, AT, None, AT,
-                           c_longlong(N if ldo is None else ldo), c_int(M), c_int(N), c_int(K))
+                           c_longlong(N if ldo is None else ldo), c_int(M), c_int(N), c_int(K), scratch, c_longlong(room))
 
 
 def _gemm8(lib, M=4, N=64, K=64, x=AT, ldo=None, xs=AT, scratch=None, room=0):
@@ -27,16 +27,26 @@ def test_products_refuse_what_their_kernels_do_not_take():
     lib = kernels.library()
     off = c_void_p((1 << 20) + 8)
     for kw in (dict(K=48), dict(K=0), dict(M=-1), dict(N=0), dict(x=off), dict(codes=off), dict(ldx=68), dict(ldx=32), dict(ldo=63), dict(dtype=2),
-               dict(M=65), dict(N=1 << 30, glu=1), dict(ldx=(1 << 24) + 8), dict(K=(1 << 24) + 32)):
+               dict(M=65), dict(N=1 << 30, glu=1), dict(ldx=(1 << 24) + 8), dict(K=(1 << 23) + 32)):
         _refused(_gemm(lib, **kw), b"ta_gemm_mx4:")
     for kw in (dict(K=48), dict(M=-1), dict(N=0), dict(x=off), dict(ldo=63), dict(M=2147483647, N=2147483647), dict(K=(1 << 23) + 32),
                dict(M=65, K=96), dict(M=65, K=96, scratch=AT, room=(65 + 64) * 16 - 1), dict(M=65, K=96, scratch=c_void_p((1 << 20) + 8), room=1 << 20),
                dict(M=65, K=512, xs=c_void_p((1 << 20) + 1))):
         _refused(_gemm8(lib, **kw), b"ta_gemm_mx4_mx8:")
     assert lib.ta_mx4_max_rows() == kernels.MX4_MAX_ROWS
-    lib.ta_gemm_mx4_mx8_scratch.restype = c_longlong
-    for M, N, K, need in ((kernels.MX8_FEW_ROWS, 70, 96, 0), (kernels.MX8_FEW_ROWS + 1, 70, 96, 135 * 16), (65, 70, 512, 0), (65, 70, 544, 135 * 32)):
-        assert lib.ta_gemm_mx4_mx8_scratch(c_int(M), c_int(N), c_int(K)) == need
+    # more rows: scratch for scales off 16 bytes, (rows of x in 8 bits and of the weights) * 16 bytes every 512 k, and for planes
+    for eight in (False, True):
+        for glu in (False, True)[:1 if eight else 2]:
+            for M, N, K, need in ((kernels.MX_FEW_ROWS, 70, 96, 0), (64, 70, 96, ((64 if eight else 0) + (140 if glu else 70)) * 16), (64, 70, 512, 0)):
+                assert kernels.gemm_mx4_scratch(eight, glu, M, N, K) == need
+        assert kernels.gemm_mx4_scratch(eight, False, 64, 64, 512, False) == (128 if eight else 64) * 16
+        need = kernels.gemm_mx4_scratch(eight, False, 33, 4096, 4096)
+        assert need and need % (33 * 4096 * 4) == 0
+        call = _gemm8 if eight else _gemm
+        name = b"ta_gemm_mx4_mx8:" if eight else b"ta_gemm_mx4:"
+        for kw in (dict(), dict(scratch=AT, room=need - 1), dict(scratch=c_void_p((1 << 20) + 8), room=need)):
+            _refused(call(lib, M=33, N=4096, K=4096, **kw), name)
+    _refused(_gemm(lib, M=64, N=(1 << 23) + 1, K=512, glu=1, scratch=AT, room=1 << 62), b"ta_gemm_mx4:")     # 4 GB of gates and ups
     assert _gemm(lib, M=0) == 0 and _gemm8(lib, M=0) == 0
 
 
@@ -72,6 +82,7 @@ def test_a_launch_without_a_device_fails():
     if torch.cuda.is_available():
         pytest.skip("the operands are addresses of nothing: only where no kernel can be launched")
     lib = kernels.library()
-    for rc, name in ((_gemm(lib), b"ta_gemm_mx4"), (_gemm(lib, glu=1, M=40), b"ta_gemm_mx4"), (_gemm8(lib), b"ta_gemm_mx4_mx8"),
-                     (_gemm8(lib, M=600, N=1024, K=2048), b"ta_gemm_mx4_mx8")):
+    room = dict(scratch=AT, room=1 << 40)
+    for rc, name in ((_gemm(lib), b"ta_gemm_mx4"), (_gemm(lib, glu=1, M=40, **room), b"ta_gemm_mx4"), (_gemm8(lib), b"ta_gemm_mx4_mx8"),
+                     (_gemm(lib, M=33, N=4096, K=4096, **room), b"ta_gemm_mx4"), (_gemm8(lib, M=600, N=1024, K=2048, **room), b"ta_gemm_mx4_mx8")):
         assert rc != 0 and lib.ta_last_error().startswith(name), lib.ta_last_error()

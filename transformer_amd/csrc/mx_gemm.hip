@@ -10,7 +10,6 @@
 // coarsely, and only the running sums over k are float32.
 #include "mx.h"
 #include <type_traits>
-#include <stdlib.h>
 
 __device__ __forceinline__ mx_bf16x8 mx_widen8(uint32_t codes, float scale) {
   union {
@@ -35,6 +34,41 @@ struct MxGemm {
   int M, N, K;
   int wide;                   // out is float32, else bfloat16
 };
+
+// COUNT neighbouring results of a row at out + at, `left` of them inside it; whole: all, and on 16 (8 where they are 4 bfloat16) bytes
+template <int COUNT>
+__device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const float* y, bool whole, int left) {
+  if (g.wide) {
+    float* o = (float*)g.out + at;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < COUNT; i += 4) *reinterpret_cast<mx_f32x4*>(o + i) = mx_f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i)
+        if (i < left) o[i] = y[i];
+    }
+    return;
+  }
+  bf16_t* o = (bf16_t*)g.out + at;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < COUNT; i += COUNT < 8 ? 4 : 8) {
+      if (COUNT < 8) {
+        *reinterpret_cast<mx_u32x2*>(o + i) = mx_u32x2{f32x2_to_bf16x2_bits(y[i], y[i + 1]), f32x2_to_bf16x2_bits(y[i + 2], y[i + 3])};
+      } else {
+        mx_u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = f32x2_to_bf16x2_bits(y[(i + 2 * j) % COUNT], y[(i + 2 * j + 1) % COUNT]);
+        *reinterpret_cast<mx_u32x4*>(o + i) = v;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      if (i < left) o[i] = from_f32<bf16_t>(y[i]);
+  }
+}
 
 // ---------------------------------------------------------------- few rows
 // A workgroup owns 16 NT rows of the weights (with GLU 8 NT gates and their ups) and all rows of x; its waves deal k out among
@@ -294,8 +328,8 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
   return ta_check_launch(what);
 }
 
-// ---------------------------------------------------------------- many 8-bit rows
-// Tiles of BM rows by BN columns, k by steps of 128 (one matrix instruction). Both operands come into LDS without registers in
+// ---------------------------------------------------------------- tiles of many rows
+// Tiles of BM rows by BN rows of the weights, k by steps of 128 (one scaled matrix instruction, or four on bfloat16). Both operands come into LDS without registers in
 // between, NS - 1 steps ahead, and so do the scales of every four steps (a row's are four bytes a step in a line of their own:
 // step by step they cost as many requests as the operands).
 //
@@ -309,10 +343,14 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
 // The weights are the first operand: a lane then holds 4 neighbouring columns of one row. Row p of the tile t of 16 stands for
 // column 16 (p / 4) + 4 t + p % 4 of the wave's 64, so a lane's four tiles are 16 neighbouring columns, stored 16 bytes at a time.
 // Pieces of 16 bytes are permuted by the row's number, so that eight lanes' reads meet no bank twice.
+// Where the tiles do not fill the CUs, k is cut among `parts` workgroups, which leave float32 sums in planes; mx_planes_kernel adds
+// them in order and finishes. GLU: a tile holds 64 gates and their 64 ups, a lane's 16 columns are then 8 of either.
 struct MxTiles {
   const uint8_t *xs, *ws;     // scales in rows of `step` bytes, a multiple of 16, 127 behind the last block
   int step;
   int m_tiles, n_tiles;
+  int parts, part_steps;      // steps of a part, a multiple of 4
+  float* planes;              // [parts][M][rows of the weights], or null
 };
 
 // 16 bytes a lane to the LDS that starts at `lds`; base and lds are the whole wave's
@@ -320,44 +358,54 @@ __device__ __forceinline__ void mx_to_lds16(const void* base, uint32_t offset, u
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "m0", "memory");
 }
 
-template <int BM, int BN, int WM, int WN, int KG, int NS>
+template <bool X8, bool GLU, int BM, int BN, int WM, int WN, int KG, int NS>
 __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
-  constexpr int W = 8, TM = BM / (16 * WM);
-  constexpr int XL = BM / 8 / W, WL = BN / 16 / W;             // loads of 1 KB a wave and step
-  constexpr int SL = (BM + BN) / 64;                           // loads of 64 rows' scales, one a wave
+  constexpr int W = 8, TM = BM / (16 * WM), XB = X8 ? 128 : 256;        // bytes of a row of x in a step
+  constexpr int XP = XB / 16, FLIP = X8 ? 7 : 15;                       // its pieces
+  constexpr int XL = BM * XB / 1024 / W, WL = BN / 16 / W;     // loads of 1 KB a wave and step
+  constexpr int SX = X8 ? BM : 0, SL = (SX + BN) / 64;         // loads of 64 rows' scales, one a wave
   constexpr int LOADS = XL + WL;
-  constexpr int AT_W = BM * 128, STAGE = AT_W + BN * 64, AT_S = NS * STAGE, GROUP = (BM + BN) * 16;
+  constexpr int AT_W = BM * XB, STAGE = AT_W + BN * 64, AT_S = NS * STAGE, GROUP = (SX + BN) * 16;
   static_assert(BN == 64 * WN && WM * WN * KG == W && BM % (16 * WM) == 0, "eight waves");
-  static_assert(XL * 8 * W == BM && WL * 16 * W == BN && SL <= W && NS <= 4, "tiles in whole loads");
+  static_assert(XL * 1024 * W == BM * XB && WL * 16 * W == BN && SL <= W && NS <= 4, "tiles in whole loads");
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, q = lane / 16;
   const int group = wave / 4, part = KG == 2 ? wave % 4 : wave, wm = part / WN, wn = part % WN;
   // workgroups go round the 8 XCDs: each gets neighbouring tiles, all rows of a band of columns, so that its cache holds them
-  const int tiles = z.m_tiles * z.n_tiles, per = tiles / 8, b = blockIdx.x;
+  const int tiles = z.m_tiles * z.n_tiles, per = tiles / 8, b = blockIdx.x % tiles, cut = blockIdx.x / tiles;
   const int tile = b < per * 8 ? (b % 8) * per + b / 8 : b;
-  const int m0 = tile % z.m_tiles * BM, n0 = tile / z.m_tiles * BN;
-  const int steps = (g.K + 127) / 128, pieces = g.K / 16, full = g.K / 128;
-  const unsigned char* x = (const unsigned char*)g.x + (size_t)m0 * g.K;
-  const unsigned char* w = g.codes + (size_t)n0 * (g.K / 2);
+  const int m0 = tile % z.m_tiles * BM, n0 = tile / z.m_tiles * (GLU ? BN / 2 : BN);
+  const int first = cut * z.part_steps, left = (g.K + 127) / 128 - first;       // this part's steps
+  const int steps = left < z.part_steps ? left : z.part_steps;
+  const int whole_steps = g.K / 128 - first, full = whole_steps < steps ? whole_steps : steps;
+  const int pieces = g.K / (X8 ? 16 : 8) - first * XP, wpieces = g.K / 32 - first * 4;
+  const unsigned char* x = (const unsigned char*)g.x + (size_t)m0 * g.ldx * (X8 ? 1 : 2) + (size_t)first * XB;
+  const unsigned char* w = g.codes + (size_t)n0 * (g.K / 2) + (size_t)first * 64;
 
   uint32_t xo[XL], wo[WL], so;
 #pragma unroll
   for (int i = 0; i < XL; ++i) {
-    const int row = (wave * XL + i) * 8 + lane / 8, piece = (lane % 8) ^ (row & 7);
-    xo[i] = (uint32_t)(m0 + row < g.M ? row : g.M - 1 - m0) * (uint32_t)g.K + piece * 16;
+    const int at = (wave * XL + i) * 64 + lane, row = at / XP, piece = (at % XP) ^ (row & FLIP);
+    xo[i] = (uint32_t)(m0 + row < g.M ? row : g.M - 1 - m0) * ((uint32_t)g.ldx * (X8 ? 1 : 2)) + piece * 16;
   }
+  // row of the weights, from n0 on, behind row `row` of the tile
+  const auto weight_row = [&](int row) {
+    if (!GLU) return (uint32_t)(n0 + row < g.N ? row : g.N - 1 - n0);
+    const int c = row / 64 * 32 + row % 64 / 16 * 8 + row % 8, up = row % 16 / 8;
+    return (uint32_t)(n0 + c < g.N ? c : g.N - 1 - n0) + (up ? (uint32_t)g.N : 0u);
+  };
 #pragma unroll
   for (int i = 0; i < WL; ++i) {
     const int row = (wave * WL + i) * 16 + lane / 4, piece = (lane % 4) ^ (row >> 4 & 3);
-    wo[i] = (uint32_t)(n0 + row < g.N ? row : g.N - 1 - n0) * (uint32_t)(g.K / 2) + piece * 16;
+    wo[i] = weight_row(row) * (uint32_t)(g.K / 2) + piece * 16;
   }
   const int sl = wave % SL;                     // waves beyond the scales' loads bring some of them once more
-  const bool s_x = sl < BM / 64;
+  const bool s_x = sl < SX / 64;
   {
-    const int row = (s_x ? sl : sl - BM / 64) * 64 + lane, last = s_x ? g.M - 1 - m0 : g.N - 1 - n0;
-    so = (uint32_t)(row < last ? row : last) * (uint32_t)z.step;
+    const int row = (s_x ? sl : sl - SX / 64) * 64 + lane;
+    so = (s_x ? (uint32_t)(m0 + row < g.M ? row : g.M - 1 - m0) : weight_row(row)) * (uint32_t)z.step;
   }
-  const unsigned char* sbase = s_x ? z.xs + (size_t)m0 * z.step : z.ws + (size_t)n0 * z.step;
+  const unsigned char* sbase = (s_x ? z.xs + (size_t)m0 * z.step : z.ws + (size_t)n0 * z.step) + (size_t)first * 4;
 
   uint32_t to_lds = 0;                          // the place of the next step asked for
   const unsigned char *xk = x, *wk = w, *sk = sbase;
@@ -376,17 +424,17 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
       // k ends inside this step: nothing behind it, zero in x, any codes in w
 #pragma unroll
       for (int i = 0; i < XL; ++i) {
-        const int row = (wave * XL + i) * 8 + lane / 8, piece = (lane % 8) ^ (row & 7);
-        if (step * 8 + piece < pieces) mx_to_lds16(xk, xo[i], to_lds + (wave * XL + i) * 1024);
+        const int at = (wave * XL + i) * 64 + lane, row = at / XP, piece = (at % XP) ^ (row & FLIP);
+        if (step * XP + piece < pieces) mx_to_lds16(xk, xo[i], to_lds + (wave * XL + i) * 1024);
         else reinterpret_cast<mx_u32x4*>(mx_lds + to_lds + (wave * XL + i) * 1024)[lane] = mx_u32x4{0, 0, 0, 0};
       }
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
         const int row = (wave * WL + i) * 16 + lane / 4, piece = (lane % 4) ^ (row >> 4 & 3);
-        if (step * 4 + piece < pieces / 2) mx_to_lds16(wk, wo[i], to_lds + AT_W + (wave * WL + i) * 1024);
+        if (step * 4 + piece < wpieces) mx_to_lds16(wk, wo[i], to_lds + AT_W + (wave * WL + i) * 1024);
       }
     }
-    xk += 128;
+    xk += XB;
     wk += 64;
     sk += 4;
     to_lds = to_lds == (NS - 1) * STAGE ? 0 : to_lds + STAGE;
@@ -400,30 +448,31 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   // With eight tiles of rows a wave, the second four are read while the first are multiplied, each in the registers that it frees
   constexpr int HELD = TM > 4 ? 4 : TM;
   static_assert(HELD == TM || KG == 1, "a step's place stays while it is multiplied");
-  mx_i32x8 wf[4], xf[HELD];
+  mx_u32x4 wf[4], xf[HELD][XP / 4];
   int ws[4], xs[HELD];
   // where a lane reads: the tiles lie a fixed number of bytes apart
   const uint32_t w_at = AT_W + (wn * 64 + 16 * (r / 4) + r % 4) * 64 + (q ^ (r / 4)) * 16;
-  const uint32_t x_at = (wm * TM * 16 + r) * 128 + (q ^ (r & 7)) * 16;
-  const uint32_t ws_at = AT_S + (BM + wn * 64 + 16 * (r / 4) + r % 4) * 16 + q, xs_at = AT_S + (wm * TM * 16 + r) * 16 + q;
+  const uint32_t x_at = (wm * TM * 16 + r) * XB;
+  const uint32_t ws_at = AT_S + (SX + wn * 64 + 16 * (r / 4) + r % 4) * 16 + q, xs_at = AT_S + (wm * TM * 16 + r) * 16 + q;
   uint32_t from = KG == 2 && group ? STAGE : 0;  // the place of the step to read
-  const unsigned char *wl, *x0, *x1, *wsl, *xsl;
+  const unsigned char *xl, *xsl;
   const auto read_x = [&](int m) {
-    const mx_u32x4 lo = *reinterpret_cast<const mx_u32x4*>(x0 + m * 2048), hi = *reinterpret_cast<const mx_u32x4*>(x1 + m * 2048);
-    xf[m % HELD] = mx_i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-    xs[m % HELD] = xsl[m * 256];
+#pragma unroll
+    for (int i = 0; i < XP / 4; ++i) {
+      // 8 bits: halves q % 2 of the blocks q / 2 and 2 + q / 2; bfloat16: the four eights of block q
+      const uint32_t piece = X8 ? (uint32_t)(q + 4 * i) ^ (r & FLIP) : (uint32_t)(4 * q + i) ^ (r & FLIP);
+      xf[m % HELD][i] = *reinterpret_cast<const mx_u32x4*>(xl + piece * 16 + m * 16 * XB);
+    }
+    if (X8) xs[m % HELD] = xsl[m * 256];
   };
   const auto read = [&](int step) {
     const uint32_t sc = (step & 4) / 4 * GROUP + (step & 3) * 4;
-    wl = mx_lds + (w_at + from);
-    x0 = mx_lds + (x_at + from);
-    x1 = mx_lds + ((x_at ^ 64) + from);
-    wsl = mx_lds + (ws_at + sc);
+    const unsigned char *wl = mx_lds + (w_at + from), *wsl = mx_lds + (ws_at + sc);
+    xl = mx_lds + (x_at + from);
     xsl = mx_lds + (xs_at + sc);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const mx_u32x4 v = *reinterpret_cast<const mx_u32x4*>(wl + t * 256);
-      wf[t] = mx_i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+      wf[t] = *reinterpret_cast<const mx_u32x4*>(wl + t * 256);
       ws[t] = wsl[t * 64];
     }
 #pragma unroll
@@ -432,20 +481,46 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
     from = from >= NS * STAGE ? from - NS * STAGE : from;
   };
   const auto multiply = [&]() {
+    if constexpr (X8) {
 #pragma unroll
-    for (int m = 0; m < TM; ++m) {
+      for (int m = 0; m < TM; ++m) {
+        const mx_u32x4 lo = xf[m % HELD][0], hi = xf[m % HELD][1];
+        const mx_i32x8 v = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        acc[m][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[t], xf[m % HELD], acc[m][t], 4, 0, 0, ws[t], 0, xs[m % HELD]);
-      if (m + HELD < TM) read_x(m + HELD);
+        for (int t = 0; t < 4; ++t) {
+          const mx_i32x8 a = {(int)wf[t][0], (int)wf[t][1], (int)wf[t][2], (int)wf[t][3], 0, 0, 0, 0};
+          acc[m][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, v, acc[m][t], 4, 0, 0, ws[t], 0, xs[m % HELD]);
+        }
+        if (m + HELD < TM) read_x(m + HELD);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float scale = mx_scale((uint32_t)ws[t]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const mx_bf16x8 a = mx_widen8(wf[t][j], scale);
+#pragma unroll
+          for (int m = 0; m < TM; ++m)
+            acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(mx_bf16x8, xf[m][j % (XP / 4)]), acc[m][t], 0, 0, 0);
+        }
+      }
     }
   };
-  // the end of a phase; `waits`: for the step that the next one reads, with NS - 2 whole ones asked for behind it, or for all
-  const auto end = [&](bool waits, bool all) {
-    if (waits) {
-      if (all) ta_wait_loads<0>();
-      else ta_wait_loads<(NS - 2) * LOADS>();
+  // the end of a phase; `next`: the step that has to be there then (none: -1), with whole steps up to `asked` asked for behind it
+  const auto end = [&](int next, int asked) {
+    if (next >= 0) {
+      const int last = asked < full ? asked : full - 1;        // (one that k ends inside of has fewer loads: it does not count)
+      if (NS > 3 && last - next >= 2) ta_wait_loads<2 * LOADS>();
+      else if (last - next >= 1) ta_wait_loads<LOADS>();
+      else ta_wait_loads<0>();
     }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto end_inside = [&](bool waits) {      // the same with NS - 2 whole steps behind the next
+    if (waits) ta_wait_loads<(NS - 2) * LOADS>();
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -455,69 +530,69 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
 
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) ask(any, i);
-  end(true, NS - 1 >= full);
+  end(0, NS - 2);
   if (KG == 1) {
     // phases 2 k and 2 k + 1: group 0 reads step k, then multiplies; group 1 multiplies step k - 1, then reads step k; in the
     // second both ask
     int k = 0;
     if (group) {
-      end(false, false);
+      end(-1, 0);
       for (; k + NS <= full; ++k) {
         ask(inside, k + NS - 1);
         read(k);
-        end(true, false);
+        end_inside(true);
         multiply();
-        end(false, false);
+        end_inside(false);
       }
       for (; k < steps; ++k) {
         ask(any, k + NS - 1);
         read(k);
-        end(true, true);
+        end(k + 1, k + NS - 1);
         multiply();
-        end(false, false);
+        end(-1, 0);
       }
     } else {
       for (; k + NS <= full; ++k) {
         read(k);
-        end(false, false);
+        end_inside(false);
         ask(inside, k + NS - 1);
         multiply();
-        end(true, false);
+        end_inside(true);
       }
       for (; k < steps; ++k) {
         read(k);
-        end(false, false);
+        end(-1, 0);
         ask(any, k + NS - 1);
         multiply();
-        end(true, true);
+        end(k + 1, k + NS - 1);
       }
-      end(false, false);
+      end(-1, 0);
     }
   } else {
     // phase p: the group p % 2 reads step p, the other multiplies step p - 1, both ask
     int p = 0;
     if (group) {
       ask(any, NS - 1);
-      end(true, NS > full);
+      end(1, NS - 1);
       p = 1;
     }
     for (; p + NS + 1 <= full; p += 2) {
       ask(inside, p + NS - 1);
       read(p);
-      end(true, false);
+      end_inside(true);
       ask(inside, p + NS);
       multiply();
-      end(true, false);
+      end_inside(true);
     }
     for (; p < steps; p += 2) {
       ask(any, p + NS - 1);
       read(p);
-      end(true, true);
+      end(p + 1, p + NS - 1);
       ask(any, p + NS);
       multiply();
-      end(true, true);
+      end(p + 2, p + NS);
     }
-    if (p == steps) end(true, true);             // as many phases for either group: the last of them was the other's
+    if (p == steps) end(-1, 0);                  // as many phases for either group: the last of them was the other's
   }
   ta_wait_loads<0>();
 
@@ -539,34 +614,90 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
       for (int t = 0; t < 4; ++t) acc[m][t] += sums[((part * TM + m) * 4 + t) * 64 + lane];
   }
 
-  const int n = n0 + wn * 64 + 16 * q;           // this lane's 16 columns
+  if (z.planes) {
+    // rows of the weights in this lane's registers: 4 t + i behind the first, with GLU 8 gates and 8 ups
+    const long long rows = GLU ? 2LL * g.N : g.N;
+    const int n = n0 + (GLU ? wn * 32 + 8 * q : wn * 64 + 16 * q);
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+      const int row = m0 + (wm * TM + m) * 16 + r;
+      if (row >= g.M) continue;
+      float* o = z.planes + ((size_t)cut * g.M + row) * rows + n;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int c = GLU ? 4 * (t % 2) : 4 * t;
+        float* to = o + c + (GLU && t >= 2 ? g.N : 0);
+        if (n + c + 4 <= g.N && rows % 4 == 0 && (!GLU || g.N % 4 == 0)) *reinterpret_cast<mx_f32x4*>(to) = acc[m][t];
+        else
+          for (int i = 0; i < 4; ++i)
+            if (n + c + i < g.N) to[i] = acc[m][t][i];
+      }
+    }
+    return;
+  }
+  constexpr int CN = GLU ? 8 : 16;               // this lane's columns of the result
+  const int n = n0 + wn * (4 * CN) + CN * q;
   float add[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) add[i] = g.bias && n + i < g.N ? g.bias[n + i] : 0.f;
-  const bool whole = n + 16 <= g.N && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0;
+  for (int i = 0; i < 16; ++i) {
+    const int c = i % CN;
+    add[i] = g.bias && n + c < g.N ? g.bias[n + c + (i >= CN ? (long long)g.N : 0)] : 0.f;
+  }
+  const int piece = g.wide ? 4 : 8;
+  const bool whole = n + CN <= g.N && g.ldo % piece == 0 && (uintptr_t)g.out % 16 == 0;
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
     const int row = m0 + (wm * TM + m) * 16 + r;
     if (row >= g.M) continue;
-    bf16_t* o = (bf16_t*)g.out + row * g.ldo + n;
-    if (whole) {
-      mx_u32x4 v[2];
+    float y[CN];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          v[t / 2][t % 2 * 2 + i] =
-              f32x2_to_bf16x2_bits(acc[m][t][2 * i] + add[4 * t + 2 * i], acc[m][t][2 * i + 1] + add[4 * t + 2 * i + 1]);
-      reinterpret_cast<mx_u32x4*>(o)[0] = v[0];
-      reinterpret_cast<mx_u32x4*>(o)[1] = v[1];
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + 4 * t + i < g.N) o[4 * t + i] = from_f32<bf16_t>(acc[m][t][i] + add[4 * t + i]);
+    for (int i = 0; i < CN; ++i) {
+      const float v = acc[m][i / 4][i % 4] + add[i];
+      if (GLU) {
+        const float u = acc[m][2 + i / 4 % 2][i % 4] + add[8 + i % 8];
+        y[i] = v / (1.0f + expf(-v)) * u;
+      } else {
+        y[i] = v;
+      }
     }
+    mx_store<CN>(g, (long long)row * g.ldo + n, y, whole, g.N - n);
   }
+}
+
+// the planes' sums in order, finished: four columns a thread
+template <bool GLU>
+__global__ __launch_bounds__(256) void mx_planes_kernel(MxGemm g, const float* __restrict__ planes, int parts) {
+  const int per = (g.N + 3) / 4;
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int row = (int)(at / per), n = (int)(at % per) * 4;
+  if (row >= g.M) return;
+  const long long rows = GLU ? 2LL * g.N : g.N, plane = (long long)g.M * rows;
+  const bool four = n + 4 <= g.N && g.N % 4 == 0;
+  float v[2][4];
+#pragma unroll
+  for (int u = 0; u < (GLU ? 2 : 1); ++u) {
+    const float* p = planes + row * rows + n + (u ? g.N : 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
+    for (int c = 0; c < parts; ++c, p += plane) {
+      if (four) {
+        const mx_f32x4 t = *reinterpret_cast<const mx_f32x4*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[u][i] += t[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[u][i] += n + i < g.N ? p[i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (g.bias && n + i < g.N) v[u][i] += g.bias[n + i + (u ? (long long)g.N : 0)];
+  }
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = GLU ? v[0][i] / (1.0f + expf(-v[0][i])) * v[1][i] : v[0][i];
+  const bool whole = n + 4 <= g.N && g.ldo % 4 == 0 && (uintptr_t)g.out % 16 == 0;
+  mx_store<4>(g, (long long)row * g.ldo + n, y, whole, g.N - n);
 }
 
 // scales of rows of `blocks` bytes into rows of `step`, 127 behind them: k that is no multiple of 512 leaves rows off the 16
@@ -584,12 +715,12 @@ __global__ __launch_bounds__(256) void mx_scales_kernel(const uint8_t* __restric
   *reinterpret_cast<uint32_t*>(to + at) = v;
 }
 
-template <int BM, int BN, int WM, int WN, int KG, int NS>
+template <bool X8, bool GLU, int BM, int BN, int WM, int WN, int KG, int NS>
 static int mx_tile_launch(const char* what, hipStream_t stream, const MxGemm& g, MxTiles z) {
-  constexpr int steps = NS * (BM * 128 + BN * 64) + 2 * (BM + BN) * 16, sums = KG == 2 ? BM * BN * 4 : 0;
+  constexpr int steps = NS * (BM * (X8 ? 128 : 256) + BN * 64) + 2 * ((X8 ? BM : 0) + BN) * 16, sums = KG == 2 ? BM * BN * 4 : 0;
   constexpr int bytes = steps > sums ? steps : sums;
   static_assert(bytes <= MX_LDS, "a workgroup's LDS");
-  const auto kernel = mx_tile_kernel<BM, BN, WM, WN, KG, NS>;
+  const auto kernel = mx_tile_kernel<X8, GLU, BM, BN, WM, WN, KG, NS>;
   static bool asked = false;
   if (!asked && bytes > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -597,8 +728,78 @@ static int mx_tile_launch(const char* what, hipStream_t stream, const MxGemm& g,
     asked = true;
   }
   z.m_tiles = (g.M + BM - 1) / BM;
-  z.n_tiles = (g.N + BN - 1) / BN;
-  kernel<<<z.m_tiles * z.n_tiles, 512, bytes, stream>>>(g, z);
+  z.n_tiles = (g.N + (GLU ? BN / 2 : BN) - 1) / (GLU ? BN / 2 : BN);
+  kernel<<<z.m_tiles * z.n_tiles * z.parts, 512, bytes, stream>>>(g, z);
+  return ta_check_launch(what);
+}
+
+// What the tiles need: which of them, in how many parts of k, and the bytes of scratch for scales and planes.
+struct MxPlan {
+  int form;                   // into mx_forms
+  int parts, part_steps;
+  bool scales;                // laid out again
+  long long scale_bytes, bytes;
+  double us;
+};
+// Tiles and what 128 k of one take while every CU has one (measured on MI355X in us: k 4,096 and 14,336, one to seven
+// rounds)
+static const struct {
+  int bm, bn;
+  double us;
+} mx_forms[] = {{64, 128, 0.40}, {128, 128, 0.62}, {128, 256, 0.93}, {256, 256, 1.60}};
+static int mx_step(int K) { return (K + 511) / 512 * 16; }
+
+static MxPlan mx_plan(bool x8, bool glu, int M, int N, int K, bool aligned) {
+  const long long rows = glu ? 2LL * N : N;
+  const int steps = (K + 127) / 128;
+  MxPlan best = {};
+  best.us = 1e30;
+  for (int f = 0; f < (x8 ? 4 : 1); ++f) {
+    const long long tiles = ((long long)M + mx_forms[f].bm - 1) / mx_forms[f].bm * ((rows + mx_forms[f].bn - 1) / mx_forms[f].bn);
+    for (int parts = 1; parts <= 16; ++parts) {
+      const int each = ((steps + parts - 1) / parts + 3) / 4 * 4;
+      if (parts > 1 && (tiles * parts > 512 || (long long)(parts - 1) * each >= steps)) break;
+      // planes are written and read once at some 4 TB/s, by a kernel of their own
+      const double planes = parts > 1 ? 2.5 + (double)parts * M * rows * 8 * 0.25e-6 : 0.;
+      const double us = (double)((tiles * parts + 255) / 256) * (each < steps ? each : steps) * mx_forms[f].us * (x8 ? 1. : 1.3) + planes;
+      if (us < best.us) best = {f, parts, each, false, 0, parts > 1 ? parts * (long long)M * rows * 4 : 0, us};
+    }
+  }
+  best.scales = K % 512 != 0 || !aligned;
+  best.scale_bytes = best.scales ? ((x8 ? (long long)M : 0) + rows) * mx_step(K) : 0;
+  best.bytes += best.scale_bytes;
+  return best;
+}
+
+template <bool X8, bool GLU>
+static int mx_tiles(const char* what, hipStream_t stream, const MxGemm& g, void* scratch, long long scratch_bytes) {
+  const bool aligned = (!X8 || (uintptr_t)g.xs % 16 == 0) && (uintptr_t)g.scales % 16 == 0;
+  const MxPlan plan = mx_plan(X8, GLU, g.M, g.N, g.K, aligned);
+  const long long rows = GLU ? 2LL * g.N : g.N;
+  TA_REQUIRE(plan.bytes == 0 || (scratch && scratch_bytes >= plan.bytes && (uintptr_t)scratch % 16 == 0),
+             "%s: %lld bytes of scratch, %lld are needed", what, scratch ? scratch_bytes : 0LL, plan.bytes);
+  TA_REQUIRE((rows + 256) * (g.K / 2) <= 0xffffffffLL || !GLU, "%s: gates and ups of %d x %d lie more than 4 GB apart", what, g.N, g.K);
+  MxTiles z = {g.xs, g.scales, g.K / MX_BLOCK, 0, 0, plan.parts, plan.part_steps, nullptr};
+  if (plan.scales) {
+    z.step = mx_step(g.K);
+    const long long xrows = X8 ? g.M : 0, grid = ((xrows + rows) * z.step / 4 + 255) / 256;
+    TA_REQUIRE(grid <= 0x7fffffffLL, "%s: M=%d N=%d K=%d: more scales than a launch holds", what, g.M, g.N, g.K);
+    mx_scales_kernel<<<(int)grid, 256, 0, stream>>>(g.xs, g.scales, (uint8_t*)scratch, xrows, xrows + rows, g.K / MX_BLOCK, z.step);
+    if (ta_check_launch(what)) return 1;
+    z.xs = (const uint8_t*)scratch;
+    z.ws = z.xs + (size_t)xrows * z.step;
+  }
+  if (plan.parts > 1) z.planes = (float*)((uint8_t*)scratch + plan.scale_bytes);
+  int rc;
+  if constexpr (!X8) rc = mx_tile_launch<false, GLU, 64, 128, 2, 2, 2, 4>(what, stream, g, z);
+  else if (plan.form == 0) rc = mx_tile_launch<true, false, 64, 128, 2, 2, 2, 4>(what, stream, g, z);
+  else if (plan.form == 1) rc = mx_tile_launch<true, false, 128, 128, 2, 2, 2, 3>(what, stream, g, z);
+  else if (plan.form == 2) rc = mx_tile_launch<true, false, 128, 256, 2, 4, 1, 3>(what, stream, g, z);
+  else rc = mx_tile_launch<true, false, 256, 256, 2, 4, 1, 3>(what, stream, g, z);
+  if (rc || plan.parts == 1) return rc;
+  const long long grid = ((long long)g.M * ((g.N + 3) / 4) + 255) / 256;
+  TA_REQUIRE(grid <= 0x7fffffffLL, "%s: M=%d N=%d are more than a launch holds", what, g.M, g.N);
+  mx_planes_kernel<GLU><<<(int)grid, 256, 0, stream>>>(g, z.planes, plan.parts);
   return ta_check_launch(what);
 }
 
@@ -612,43 +813,48 @@ static int mx_gemm_check(const char* what, const MxGemm& g) {
   return 0;
 }
 
+// Rows up to which the waves along k have it, by GPU time against the tiles'.
+static bool mx_few(bool x8, bool glu, int M, int N, int K) {
+  (void)x8; (void)glu; (void)N; (void)K;
+  return M <= 16;
+}
+
+// Bytes of scratch for M rows in 8 bits (x8) or bfloat16; aligned: all scales start on 16 bytes.
+extern "C" long long ta_gemm_mx4_scratch(int x8, int swiglu, int M, int N, int K, int aligned) {
+  if (M <= 0 || N <= 0 || K < MX_BLOCK || mx_few(x8, swiglu, M, N, K)) return 0;
+  return mx_plan(x8, swiglu, M, N, K, aligned).bytes;
+}
+
 // bfloat16 rows x [M][ldx] (rows on 16 bytes), at most ta_mx4_max_rows of them; out_dtype float32 or bfloat16; swiglu: the weights are N
-// gate rows and N up rows.
+// gate rows and N up rows. scratch: ta_gemm_mx4_scratch bytes on 16.
 #define MX_FEW_ROWS 64
 extern "C" int ta_mx4_max_rows() { return MX_FEW_ROWS; }
 extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const void* x, long long ldx, const void* codes, const void* scales,
-                           const float* bias, void* out, long long ldo, int M, int N, int K) {
-  TA_REQUIRE(out_dtype == TA_F32 || out_dtype == TA_BF16, "ta_gemm_mx4: unknown dtype %d", out_dtype);
+                           const float* bias, void* out, long long ldo, int M, int N, int K, void* scratch, long long scratch_bytes) {
+  static const char what[] = "ta_gemm_mx4";
+  TA_REQUIRE(out_dtype == TA_F32 || out_dtype == TA_BF16, "%s: unknown dtype %d", what, out_dtype);
   const MxGemm g = {x, nullptr, (const uint8_t*)codes, (const uint8_t*)scales, bias, out, ldx, ldo, M, N, K, out_dtype == TA_F32};
-  if (mx_gemm_check("ta_gemm_mx4", g)) return 1;
-  TA_REQUIRE(M <= MX_FEW_ROWS, "ta_gemm_mx4: %d bfloat16 rows, at most %d", M, MX_FEW_ROWS);
-  TA_REQUIRE(ldx >= K && ldx % 8 == 0, "ta_gemm_mx4: rows %lld apart do not start on 16 bytes", ldx);
-  TA_REQUIRE(ldx <= 1 << 24 && K <= 1 << 24, "ta_gemm_mx4: rows %lld apart, k %d: at most 16,777,216", ldx, K);   // 64 rows within 31 bits
-  TA_REQUIRE(!swiglu || N <= 0x3fffffff, "ta_gemm_mx4: %d gates", N);
+  if (mx_gemm_check(what, g)) return 1;
+  TA_REQUIRE(M <= MX_FEW_ROWS, "%s: %d bfloat16 rows, at most %d", what, M, MX_FEW_ROWS);
+  TA_REQUIRE(ldx >= K && ldx % 8 == 0, "%s: rows %lld apart do not start on 16 bytes", what, ldx);
+  TA_REQUIRE(ldx <= 1 << 24 && K <= 1 << 23, "%s: rows %lld apart, k %d: at most 16,777,216 and 8,388,608", what, ldx, K);   // a tile's rows within 32 bits
+  TA_REQUIRE(!swiglu || N <= 0x3fffffff, "%s: %d gates", what, N);
   if (M == 0) return 0;
+  if (!mx_few(false, swiglu, M, N, K))
+    return swiglu ? mx_tiles<false, true>(what, stream, g, scratch, scratch_bytes) : mx_tiles<false, false>(what, stream, g, scratch, scratch_bytes);
   if (swiglu) {
-    if (M <= 1) return mx_few_launch<false, true, 1, 2, 2, 1>("ta_gemm_mx4", stream, g);
-    if (M <= 4) return mx_few_launch<false, true, 1, 2, 2, 4>("ta_gemm_mx4", stream, g);
-    if (M <= 8) return mx_few_launch<false, true, 1, 2, 2, 8>("ta_gemm_mx4", stream, g);
-    if (M <= 16) return mx_few_launch<false, true, 1, 2, 2, 16>("ta_gemm_mx4", stream, g);
-    if (M <= 32) return mx_few_launch<false, true, 2, 2, 2, 32>("ta_gemm_mx4", stream, g);
-    return mx_few_launch<false, true, 4, 2, 2, 64>("ta_gemm_mx4", stream, g);
+    if (M <= 1) return mx_few_launch<false, true, 1, 2, 2, 1>(what, stream, g);
+    if (M <= 4) return mx_few_launch<false, true, 1, 2, 2, 4>(what, stream, g);
+    if (M <= 8) return mx_few_launch<false, true, 1, 2, 2, 8>(what, stream, g);
+    return mx_few_launch<false, true, 1, 2, 2, 16>(what, stream, g);
   }
-  if (M <= 1) return mx_few_launch<false, false, 1, 1, 4, 1>("ta_gemm_mx4", stream, g);
-  if (M <= 4) return mx_few_launch<false, false, 1, 1, 4, 4>("ta_gemm_mx4", stream, g);
-  if (M <= 8) return mx_few_launch<false, false, 1, 1, 4, 8>("ta_gemm_mx4", stream, g);
-  if (M <= 16) return mx_few_launch<false, false, 1, 1, 2, 16>("ta_gemm_mx4", stream, g);
-  if (M <= 32) return mx_few_launch<false, false, 2, 2, 2, 32>("ta_gemm_mx4", stream, g);
-  return mx_few_launch<false, false, 4, 2, 2, 64>("ta_gemm_mx4", stream, g);
+  if (M <= 1) return mx_few_launch<false, false, 1, 1, 4, 1>(what, stream, g);
+  if (M <= 4) return mx_few_launch<false, false, 1, 1, 4, 4>(what, stream, g);
+  if (M <= 8) return mx_few_launch<false, false, 1, 1, 4, 8>(what, stream, g);
+  return mx_few_launch<false, false, 1, 1, 2, 16>(what, stream, g);
 }
 
-// 8-bit rows, codes [M][K] and bytes [M][K/32]; out bfloat16. scratch: ta_gemm_mx4_mx8_scratch bytes on 16 (0: null will do
-// where the scales start on 16 bytes).
-#define MX_FEW_ROWS8 64
-static int mx_step(int K) { return (K + 511) / 512 * 16; }
-extern "C" long long ta_gemm_mx4_mx8_scratch(int M, int N, int K) {
-  return M > MX_FEW_ROWS8 && (K % 512 != 0) ? ((long long)M + N) * mx_step(K) : 0;
-}
+// 8-bit rows, codes [M][K] and bytes [M][K/32]; out bfloat16. scratch: ta_gemm_mx4_scratch bytes on 16.
 extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs, const void* codes, const void* scales, const float* bias,
                                void* out, long long ldo, int M, int N, int K, void* scratch, long long scratch_bytes) {
   static const char what[] = "ta_gemm_mx4_mx8";
@@ -656,38 +862,9 @@ extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs
   if (mx_gemm_check(what, g)) return 1;
   TA_REQUIRE(K <= 1 << 23, "%s: k %d: at most 8,388,608", what, K);         // 256 rows within 31 bits
   if (M == 0) return 0;
+  if (!mx_few(true, false, M, N, K)) return mx_tiles<true, false>(what, stream, g, scratch, scratch_bytes);
   if (M <= 1) return mx_few_launch<true, false, 1, 1, 4, 1>(what, stream, g);
   if (M <= 4) return mx_few_launch<true, false, 1, 1, 4, 4>(what, stream, g);
   if (M <= 8) return mx_few_launch<true, false, 1, 1, 4, 8>(what, stream, g);
-  if (M <= 16) return mx_few_launch<true, false, 1, 1, 4, 16>(what, stream, g);
-  if (M <= 32) return mx_few_launch<true, false, 2, 2, 2, 32>(what, stream, g);
-  if (M <= MX_FEW_ROWS8) return mx_few_launch<true, false, 4, 2, 2, 64>(what, stream, g);
-  MxTiles z = {g.xs, g.scales, K / MX_BLOCK, 0, 0};
-  if (K % 512 || (uintptr_t)xs % 16 || (uintptr_t)scales % 16) {
-    z.step = mx_step(K);
-    const long long need = ((long long)M + N) * z.step, grid = (need / 4 + 255) / 256;
-    TA_REQUIRE(scratch && scratch_bytes >= need && (uintptr_t)scratch % 16 == 0, "%s: %lld bytes of scratch, %lld are needed", what,
-               scratch ? scratch_bytes : 0LL, need);
-    TA_REQUIRE(grid <= 0x7fffffffLL, "%s: M=%d N=%d K=%d: more scales than a launch holds", what, M, N, K);
-    mx_scales_kernel<<<(int)grid, 256, 0, stream>>>(g.xs, g.scales, (uint8_t*)scratch, M, (long long)M + N, K / MX_BLOCK, z.step);
-    if (ta_check_launch(what)) return 1;
-    z.xs = (const uint8_t*)scratch;
-    z.ws = z.xs + (size_t)M * z.step;
-  }
-  const long long big = (((long long)M + 255) / 256) * (((long long)N + 255) / 256);
-  const long long mid = (((long long)M + 127) / 128) * (((long long)N + 127) / 128);
-  if (const char* e = getenv("MXT")) switch (atoi(e)) {
-    case 1: return mx_tile_launch<64, 128, 2, 2, 2, 3>(what, stream, g, z);
-    case 2: return mx_tile_launch<64, 128, 2, 2, 2, 4>(what, stream, g, z);
-    case 4: return mx_tile_launch<128, 128, 2, 2, 2, 3>(what, stream, g, z);
-    case 5: return mx_tile_launch<128, 128, 2, 2, 2, 4>(what, stream, g, z);
-    case 6: return mx_tile_launch<128, 256, 2, 4, 1, 3>(what, stream, g, z);
-    case 8: return mx_tile_launch<256, 256, 2, 4, 1, 3>(what, stream, g, z);
-    case 9: return mx_tile_launch<256, 128, 4, 2, 1, 3>(what, stream, g, z);
-    case 11: return mx_tile_launch<128, 128, 4, 2, 1, 3>(what, stream, g, z);
-    case 12: return mx_tile_launch<64, 128, 4, 2, 1, 4>(what, stream, g, z);
-  }
-  if (big >= 256) return mx_tile_launch<256, 256, 2, 4, 1, 3>(what, stream, g, z);
-  if (mid >= 256) return mx_tile_launch<128, 128, 2, 2, 2, 3>(what, stream, g, z);
-  return mx_tile_launch<64, 128, 2, 2, 2, 3>(what, stream, g, z);
+  return mx_few_launch<true, false, 1, 1, 4, 16>(what, stream, g);
 }

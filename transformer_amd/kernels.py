@@ -2873,23 +2873,30 @@ def memory_step(proj: torch.Tensor, offsets: Sequence[int], i_bias, f_bias, cap:
 # ------------------------------------------------------------------ 4-bit weights, 8-bit rows
 # Blocks of 32 values along a row share a power of two 2^(b - 127), b a byte (255: the block is NaN). The scale of a block
 # is the smallest power of two with which its largest magnitude is at most the codes' largest value, 6 or 448.
+#
+# These launches are as short as the Python in front of them: the argument types of a function are named once, so that a call
+# hands over plain numbers, and what a call is given is checked in one expression, taken apart only for the message of a refusal.
 MX_BLOCK = 32
-_mx_types = {}
+_p, _i, _l = c_void_p, c_int, c_longlong
+_MX_TYPES = {
+    "ta_mx4_pack": (_p, _i, _p, _l, _p, _p, _l, _i),
+    "ta_mx4_unpack": (_p, _i, _p, _p, _p, _l, _l, _i),
+    "ta_mx8_pack": (_p, _i, _p, _l, _p, _p, _l, _i),
+    "ta_swiglu_mx8": (_p, _i, _p, _l, _p, _p, _p, _l, _i),
+    "ta_add_rmsnorm_mx8": (_p, _i, _p, _p, _i, _p, _p, c_float, _p, _p, _p, _i, _i),
+    "ta_gemm_mx4": (_p, _i, _i, _p, _l, _p, _p, _p, _p, _l, _i, _i, _i, _p, _l),
+    "ta_gemm_mx4_mx8": (_p, _p, _p, _p, _p, _p, _p, _l, _i, _i, _i, _p, _l),
+}
+_mx_ready = {}
 
 
-def _mx(name: str, *types):
-    """The library's function with its argument types named once, so that a call hands over plain numbers: these launches are
-    as short as the Python in front of them."""
-    f = _mx_types.get(name)
+def _mx(name: str):
+    f = _mx_ready.get(name)
     if f is None:
         f = getattr(library(), name)
-        f.argtypes, f.restype = types, c_int
-        _mx_types[name] = f
+        f.argtypes, f.restype = _MX_TYPES[name], c_int
+        _mx_ready[name] = f
     return f
-
-
-def _mx_stream():
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _here(what: str, *tensors):
@@ -2900,6 +2907,18 @@ def _here(what: str, *tensors):
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{at}")
 
 
+def _vector(t: Optional[torch.Tensor], n: int, at: int) -> bool:
+    """Whether t is None or n float32 values in a row on the current device ``at``."""
+    return t is None or (t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == at)
+
+
+def _refuse_vector(what: str, name: str, t: Optional[torch.Tensor], n: int):
+    if t is not None:
+        _dev(t, name, torch.float32)
+        if t.numel() != n:
+            raise KernelError(f"{what}: {name} must hold {n} values, one per column or row of the weights, got {t.numel()}")
+
+
 class Mx4:
     """A matrix of 4-bit weights [n, k]: ``codes`` uint8 [n, k/2], two e2m1 values to a byte (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a
     sign), the first in the low half; ``scales`` uint8 [n, k/32]. It stands where a weight tensor does."""
@@ -2907,14 +2926,15 @@ class Mx4:
     dtype = "mx4"                       # no torch.dtype: what asks for one finds another
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.dim() == 2 and codes.is_contiguous() \
+                and scales.is_contiguous() and codes.is_cuda and codes.get_device() == scales.get_device():
+            n, half = codes.shape
+            if half and half % 16 == 0 and scales.shape == (n, half // 16) and codes.data_ptr() % 16 == 0:
+                self.codes, self.scales, self.shape = codes, scales, (n, 2 * half)
+                return
         _dev(codes, "codes", torch.uint8); _dev(scales, "scales", torch.uint8)
-        if codes.dim() != 2 or codes.shape[1] % 16 or codes.shape[1] < 16 or \
-                tuple(scales.shape) != (codes.shape[0], codes.shape[1] // 16):
-            raise KernelError(f"Mx4: codes {tuple(codes.shape)} / scales {tuple(scales.shape)}: rows go by blocks of {MX_BLOCK} "
-                              f"values, 16 bytes and one scale each")
-        if codes.data_ptr() % 16 or codes.get_device() != scales.get_device():
-            raise KernelError("Mx4: codes start on 16 bytes, beside their scales on one device")
-        self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], codes.shape[1] * 2)
+        raise KernelError(f"Mx4: codes {tuple(codes.shape)} / scales {tuple(scales.shape)}: rows go by blocks of {MX_BLOCK} values, "
+                          f"16 bytes and one scale each, and start on 16 bytes, beside their scales on one device")
 
     @classmethod
     def empty(cls, n: int, k: int, device) -> "Mx4":
@@ -2937,14 +2957,15 @@ class Mx8:
     dtype = "mx8"
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype is torch.float8_e4m3fn and scales.dtype is torch.uint8 and codes.dim() == 2 and codes.is_contiguous() \
+                and scales.is_contiguous() and codes.is_cuda and codes.get_device() == scales.get_device():
+            m, k = codes.shape
+            if k and k % MX_BLOCK == 0 and scales.shape == (m, k // MX_BLOCK) and codes.data_ptr() % 16 == 0:
+                self.codes, self.scales, self.shape = codes, scales, (m, k)
+                return
         _dev(codes, "codes", torch.float8_e4m3fn); _dev(scales, "scales", torch.uint8)
-        if codes.dim() != 2 or codes.shape[1] % MX_BLOCK or codes.shape[1] < MX_BLOCK or \
-                tuple(scales.shape) != (codes.shape[0], codes.shape[1] // MX_BLOCK):
-            raise KernelError(f"Mx8: codes {tuple(codes.shape)} / scales {tuple(scales.shape)}: rows go by blocks of {MX_BLOCK} "
-                              f"values and one scale each")
-        if codes.data_ptr() % 16 or codes.get_device() != scales.get_device():
-            raise KernelError("Mx8: codes start on 16 bytes, beside their scales on one device")
-        self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], codes.shape[1])
+        raise KernelError(f"Mx8: codes {tuple(codes.shape)} / scales {tuple(scales.shape)}: rows go by blocks of {MX_BLOCK} values "
+                          f"and one scale each, and start on 16 bytes, beside their scales on one device")
 
     @classmethod
     def empty(cls, m: int, k: int, device) -> "Mx8":
@@ -2966,8 +2987,7 @@ def mx4_pack(w: torch.Tensor, out: Mx4) -> Mx4:
     if tuple(w.shape) != out.shape:
         raise KernelError(f"mx4_pack: w {tuple(w.shape)} out {out.shape}")
     _here("mx4_pack", w, out.codes)
-    f = _mx("ta_mx4_pack", c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int)
-    _check(f(_mx_stream(), _code(w.dtype), w.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), n, w.shape[1]))
+    _check(_mx("ta_mx4_pack")(_stream(), _code(w.dtype), w.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), n, w.shape[1]))
     return out
 
 
@@ -2978,8 +2998,7 @@ def mx4_unpack(w: Mx4, out: torch.Tensor) -> torch.Tensor:
     if tuple(out.shape) != w.shape:
         raise KernelError(f"mx4_unpack: w {w.shape} out {tuple(out.shape)}")
     _here("mx4_unpack", out, w.codes)
-    f = _mx("ta_mx4_unpack", c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int)
-    _check(f(_mx_stream(), _code(out.dtype), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ld, n, w.shape[1]))
+    _check(_mx("ta_mx4_unpack")(_stream(), _code(out.dtype), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ld, n, w.shape[1]))
     return out
 
 
@@ -2991,26 +3010,26 @@ def mx8_pack(x: torch.Tensor, out: Mx8) -> Mx8:
     if tuple(x.shape) != out.shape:
         raise KernelError(f"mx8_pack: x {tuple(x.shape)} out {out.shape}")
     _here("mx8_pack", x, out.codes)
-    f = _mx("ta_mx8_pack", c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_int)
-    _check(f(_mx_stream(), _code(x.dtype), x.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), m, x.shape[1]))
+    _check(_mx("ta_mx8_pack")(_stream(), _code(x.dtype), x.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), m, x.shape[1]))
     return out
 
 
 def swiglu_mx8(gate_up: torch.Tensor, out: Mx8, bias: Optional[torch.Tensor] = None) -> Mx8:
     """``swiglu`` in 32 bits with the result left as 8-bit rows: gate_up [m, 2*di] float32 or bfloat16, out [m, di]."""
-    _dev(gate_up, "gate_up", contiguous=False)
-    m, ld = _rows2d(gate_up, "gate_up")
-    d = out.shape[1]
-    if tuple(gate_up.shape) != (out.shape[0], 2 * d):
+    m, d = out.shape
+    at = torch._C._cuda_getDevice()
+    if gate_up.shape != (m, 2 * d) or gate_up.get_device() != at or out.codes.get_device() != at or not _vector(bias, 2 * d, at):
+        _dev(gate_up, "gate_up", contiguous=False)
+        _refuse_vector("swiglu_mx8", "bias", bias, 2 * d)
+        _here("swiglu_mx8", gate_up, out.codes, bias)
         raise KernelError(f"swiglu_mx8: gate_up {tuple(gate_up.shape)} / out {out.shape}")
-    if bias is not None:
-        _dev(bias, "bias", torch.float32)
-        if bias.numel() != 2 * d:
-            raise KernelError("swiglu_mx8: bias must hold one entry per gate_up column")
-    _here("swiglu_mx8", gate_up, out.codes, bias)
-    f = _mx("ta_swiglu_mx8", c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_int)
-    _check(f(_mx_stream(), _code(gate_up.dtype), gate_up.data_ptr(), ld, None if bias is None else bias.data_ptr(),
-             out.codes.data_ptr(), out.scales.data_ptr(), m, d))
+    ld, inner = gate_up.stride()
+    if inner != 1:
+        _rows2d(gate_up, "gate_up")
+    rc = _mx("ta_swiglu_mx8")(torch._C._cuda_getCurrentRawStream(at), _code(gate_up.dtype), gate_up.data_ptr(), ld,
+                              None if bias is None else bias.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d)
+    if rc:
+        _check(rc)
     return out
 
 
@@ -3019,89 +3038,112 @@ def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8,
     """``add_rmsnorm`` with the normed rows left in 8 bits: v = x + delta + delta_bias goes back to x (to ``stream`` where one
     is given, which then gets v also when nothing is added), rmsnorm(v) * weight to out. delta float32 or bfloat16 [m, d], or
     [planes, m, d] whose planes are added in order."""
-    _dev(x, "x", torch.float32); _dev(weight, "weight", torch.float32)
     m, d = out.shape
-    if tuple(x.shape) != (m, d) or weight.numel() != d:
-        raise KernelError(f"add_rmsnorm_mx8: x {tuple(x.shape)} weight {tuple(weight.shape)} out {out.shape}")
-    code, planes = F32, 0
-    if delta is not None:
-        _dev(delta, "delta")
-        if delta.shape[-2:] != x.shape or delta.dim() not in (2, 3):
-            raise KernelError(f"add_rmsnorm_mx8: delta is {tuple(delta.shape)}, x is {tuple(x.shape)}")
-        code, planes = _code(delta.dtype), 1 if delta.dim() == 2 else delta.shape[0]
-        if planes < 1:
-            raise KernelError("add_rmsnorm_mx8: delta has no planes")
-    if delta_bias is not None:
-        _dev(delta_bias, "delta_bias", torch.float32)
-        if delta_bias.numel() != d:
-            raise KernelError("add_rmsnorm_mx8: delta_bias must have one entry per column")
-    if stream is not None:
-        _dev(stream, "stream", torch.float32)
-        if stream.shape != x.shape:
-            raise KernelError(f"add_rmsnorm_mx8: stream is {tuple(stream.shape)}, x is {tuple(x.shape)}")
-    elif delta is not None or delta_bias is not None:
+    at = torch._C._cuda_getDevice()
+    code = planes = dp = 0
+    if stream is None and (delta is not None or delta_bias is not None):
         stream = x
-    _here("add_rmsnorm_mx8", x, weight, out.codes, delta, delta_bias, stream)
-    f = _mx("ta_add_rmsnorm_mx8", c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
-            c_int, c_int)
-    _check(f(_mx_stream(), code, x.data_ptr(), None if delta is None or m == 0 else delta.data_ptr(), planes if m else 0,
-             None if delta_bias is None else delta_bias.data_ptr(), weight.data_ptr(), eps,
-             None if stream is None else stream.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d))
+    ok = x.dtype is torch.float32 and x.shape == (m, d) and x.is_contiguous() and x.get_device() == at and out.codes.get_device() == at \
+        and weight is not None and _vector(weight, d, at) and _vector(delta_bias, d, at) \
+        and (stream is None or stream is x or (stream.shape == (m, d) and _vector(stream, m * d, at)))
+    if ok and delta is not None:
+        code, planes, dp = _code(delta.dtype), 1, delta.data_ptr()
+        ok = delta.is_contiguous() and delta.get_device() == at
+        if delta.shape != (m, d):
+            planes = delta.shape[0] if delta.dim() == 3 else 0
+            ok = ok and planes > 0 and delta.shape[1:] == (m, d)
+    if not ok:
+        _dev(x, "x", torch.float32); _dev(weight, "weight", torch.float32)
+        if x.shape != (m, d) or weight.numel() != d:
+            raise KernelError(f"add_rmsnorm_mx8: x {tuple(x.shape)} weight {tuple(weight.shape)} out {out.shape}")
+        _refuse_vector("add_rmsnorm_mx8", "delta_bias", delta_bias, d)
+        for t, name in ((delta, "delta"), (stream, "stream")):
+            if t is not None:
+                _dev(t, name, torch.float32 if name == "stream" else None)
+        _here("add_rmsnorm_mx8", x, weight, out.codes, delta, delta_bias, stream)
+        raise KernelError(f"add_rmsnorm_mx8: x is {tuple(x.shape)}, delta {None if delta is None else tuple(delta.shape)}, "
+                          f"stream {None if stream is None else tuple(stream.shape)}")
+    if m == 0:
+        return out
+    rc = _mx("ta_add_rmsnorm_mx8")(torch._C._cuda_getCurrentRawStream(at), code, x.data_ptr(), dp or None, planes,
+                                   None if delta_bias is None else delta_bias.data_ptr(), weight.data_ptr(), eps,
+                                   None if stream is None else stream.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d)
+    if rc:
+        _check(rc)
     return out
 
 
 MX4_MAX_ROWS = 64       # bfloat16 rows that ``gemm_mx4`` takes (ta_mx4_max_rows)
-MX8_FEW_ROWS = 64       # 8-bit rows up to which it goes without scratch (MX_FEW_ROWS8 of csrc/mx_gemm.hip)
+_mx_scratch_sizes = {}
+
+
+def gemm_mx4_scratch(eight: bool, swiglu: bool, rows: int, n: int, k: int, aligned: bool = True) -> int:
+    """Bytes of scratch that ``gemm_mx4`` allocates for a call (n: columns of the result; aligned: scales on 16 bytes)."""
+    key = (eight, swiglu, rows, n, k, aligned)
+    need = _mx_scratch_sizes.get(key)
+    if need is None:
+        f = library().ta_gemm_mx4_scratch
+        f.restype = c_longlong
+        if len(_mx_scratch_sizes) > 4096:
+            _mx_scratch_sizes.clear()
+        need = _mx_scratch_sizes[key] = int(f(c_int(eight), c_int(swiglu), c_int(rows), c_int(n), c_int(k), c_int(aligned)))
+    return need
+
+
+MX_FEW_ROWS = 16        # rows up to which no call needs any
+
 
 
 def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, swiglu: bool = False) -> torch.Tensor:
     """out = a @ w.T (+ bias) with 4-bit weights, sums in float32.
 
     a bfloat16, at most ``MX4_MAX_ROWS`` rows (more: ``mx4_unpack`` and a product of many bfloat16 rows): the weights enter with
-    their exact values (one of 2^128 and more, which bfloat16 does not hold, as an infinity), out float32 or bfloat16. swiglu: w is [2*n, k] (gate rows, up rows) and out [m, n] = silu(a @ gate.T) *
-    (a @ up.T).
+    their exact values (one of 2^128 and more, which bfloat16 does not hold, as an infinity), out float32 or bfloat16. swiglu: w
+    is [2*n, k] (gate rows, up rows) and out [m, n] = silu(a @ gate.T) * (a @ up.T).
 
     a ``Mx8``, any number of rows: the matrix cores multiply both as they are, and keep some 15 bits below the largest of
     the 128 products that they add at a time; out bfloat16."""
-    if not isinstance(w, Mx4):
+    if type(w) is not Mx4:
         raise KernelError(f"gemm_mx4: the weights are an Mx4, not {type(w).__name__}")
     n, k = w.shape
-    if isinstance(a, Mx8):
-        _dev(out, "out", torch.bfloat16, contiguous=False)
-        if swiglu:
-            raise KernelError("gemm_mx4: 8-bit rows leave gates and ups to swiglu_mx8")
-    else:
-        _dev(a, "a", torch.bfloat16, contiguous=False); _dev(out, "out", contiguous=False)
-        if swiglu and n % 2:
-            raise KernelError(f"gemm_mx4: {n} rows of weights are not gates and ups")
+    eight = type(a) is Mx8
+    x = a.codes if eight else a
+    at = torch._C._cuda_getDevice()
     m = a.shape[0]
-    mo, ldo = _rows2d(out, "out")
     cols = n // 2 if swiglu else n
-    if a.shape[1] != k or mo != m or out.shape[1] != cols:
+    wide = out.dtype is torch.float32
+    if x.shape != (m, k) or out.shape != (m, cols) or x.get_device() != at or out.get_device() != at or w.codes.get_device() != at \
+            or not (eight or x.dtype is torch.bfloat16) or not (out.dtype is torch.bfloat16 or (wide and not eight)) \
+            or (swiglu and (eight or n % 2)) or not _vector(bias, n, at):
+        _dev(x, "a", None if eight else torch.bfloat16, contiguous=False)
+        _dev(out, "out", torch.bfloat16 if eight else None, contiguous=False)
+        _refuse_vector("gemm_mx4", "bias", bias, n)
+        _here("gemm_mx4", x, w.codes, out, bias)
+        _code(out.dtype)
+        if swiglu:
+            raise KernelError("gemm_mx4: 8-bit rows leave gates and ups to swiglu_mx8" if eight else
+                              f"gemm_mx4: a {tuple(a.shape)} gates and ups {w.shape} out {tuple(out.shape)}")
         raise KernelError(f"gemm_mx4: a {tuple(a.shape)} w {w.shape} out {tuple(out.shape)}")
-    if bias is not None:
-        _dev(bias, "bias", torch.float32)
-        if bias.numel() != n:
-            raise KernelError("gemm_mx4: bias must hold one entry per row of w")
+    ldx, inner = x.stride()
+    ldo, inner_o = out.stride()
+    if inner != 1 or inner_o != 1:
+        _rows2d(x, "a"); _rows2d(out, "out")
     if m == 0 or cols == 0:
         return out
-    bp = None if bias is None else bias.data_ptr()
-    if isinstance(a, Mx8):
-        _here("gemm_mx4", a.codes, w.codes, out, bias)
-        f = _mx("ta_gemm_mx4_mx8", c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int,
-                c_void_p, c_longlong)
-        xs, ws = a.scales.data_ptr(), w.scales.data_ptr()
-        scratch, need = None, 0
-        if m > MX8_FEW_ROWS and (k % 512 or (xs | ws) % 16):    # scales whose rows are off 16 bytes are laid out again
-            need = (m + n) * (-(-k // 512) * 16)
-            scratch = torch.empty(need, dtype=torch.uint8, device=out.device)
-        _check(f(_mx_stream(), a.codes.data_ptr(), xs, w.codes.data_ptr(), ws, bp, out.data_ptr(), ldo, m, cols, k,
-                 None if scratch is None else scratch.data_ptr(), need))
-        return out
-    _here("gemm_mx4", a, w.codes, out, bias)
-    _, lda = _rows2d(a, "a")
-    f = _mx("ta_gemm_mx4", c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int,
-            c_int)
-    _check(f(_mx_stream(), _code(out.dtype), int(swiglu), a.data_ptr(), lda, w.codes.data_ptr(), w.scales.data_ptr(), bp, out.data_ptr(), ldo,
-             m, cols, k))
+    xs, ws = a.scales.data_ptr() if eight else 0, w.scales.data_ptr()
+    scratch = need = 0
+    if m > MX_FEW_ROWS:
+        need = gemm_mx4_scratch(eight, swiglu, m, cols, k, (xs | ws) % 16 == 0)
+        if need:        # the allocator's, so that calls on two streams, or two recorded graphs, do not share it
+            room = torch.empty(need, dtype=torch.uint8, device=out.device)
+            scratch = room.data_ptr()
+    stream, bp = torch._C._cuda_getCurrentRawStream(at), None if bias is None else bias.data_ptr()
+    if eight:
+        rc = _mx("ta_gemm_mx4_mx8")(stream, x.data_ptr(), xs, w.codes.data_ptr(), ws, bp, out.data_ptr(), ldo, m, cols, k, scratch or None,
+                                    need)
+    else:
+        rc = _mx("ta_gemm_mx4")(stream, 0 if wide else 1, 1 if swiglu else 0, x.data_ptr(), ldx, w.codes.data_ptr(), ws, bp, out.data_ptr(),
+                                ldo, m, cols, k, scratch or None, need)
+    if rc:
+        _check(rc)
     return out
