@@ -37,15 +37,17 @@ def test_products_refuse_what_their_kernels_do_not_take():
     # more rows: scratch for scales off 16 bytes, (rows of x in 8 bits and of the weights) * 16 bytes every 512 k, and for planes
     for eight in (False, True):
         for glu in (False, True)[:1 if eight else 2]:
-            for M, N, K, need in ((kernels.MX_FEW_ROWS, 70, 96, 0), (64, 70, 96, ((64 if eight else 0) + (140 if glu else 70)) * 16), (64, 70, 512, 0)):
-                assert kernels.gemm_mx4_scratch(eight, glu, M, N, K) == need
-        assert kernels.gemm_mx4_scratch(eight, False, 64, 64, 512, False) == (128 if eight else 64) * 16
-        need = kernels.gemm_mx4_scratch(eight, False, 33, 4096, 4096)
-        assert need and need % (33 * 4096 * 4) == 0
+            for M, N, K, need in ((kernels.MX_FEW_ROWS, 70, 96, 0), (200, 70, 96, ((200 if eight else 0) + (140 if glu else 70)) * 16), (200, 70, 512, 0)):
+                if eight:
+                    assert kernels.gemm_mx4_scratch(eight, glu, M, N, K) == need
+        if eight:
+            assert kernels.gemm_mx4_scratch(eight, False, 200, 64, 512, False) == 264 * 16
+        need = kernels.gemm_mx4_scratch(eight, False, 64, 4096, 14336)
+        assert need and need % (64 * 4096 * 4) == 0
         call = _gemm8 if eight else _gemm
         name = b"ta_gemm_mx4_mx8:" if eight else b"ta_gemm_mx4:"
         for kw in (dict(), dict(scratch=AT, room=need - 1), dict(scratch=c_void_p((1 << 20) + 8), room=need)):
-            _refused(call(lib, M=33, N=4096, K=4096, **kw), name)
+            _refused(call(lib, M=64, N=4096, K=14336, **kw), name)
     _refused(_gemm(lib, M=64, N=(1 << 23) + 1, K=512, glu=1, scratch=AT, room=1 << 62), b"ta_gemm_mx4:")     # 4 GB of gates and ups
     assert _gemm(lib, M=0) == 0 and _gemm8(lib, M=0) == 0
 
@@ -84,5 +86,5 @@ def test_a_launch_without_a_device_fails():
     lib = kernels.library()
     room = dict(scratch=AT, room=1 << 40)
     for rc, name in ((_gemm(lib), b"ta_gemm_mx4"), (_gemm(lib, glu=1, M=40, **room), b"ta_gemm_mx4"), (_gemm8(lib), b"ta_gemm_mx4_mx8"),
-                     (_gemm(lib, M=33, N=4096, K=4096, **room), b"ta_gemm_mx4"), (_gemm8(lib, M=600, N=1024, K=2048, **room), b"ta_gemm_mx4_mx8")):
+                     (_gemm(lib, M=64, N=4096, K=14336, **room), b"ta_gemm_mx4"), (_gemm8(lib, M=600, N=1024, K=2048, **room), b"ta_gemm_mx4_mx8")):
         assert rc != 0 and lib.ta_last_error().startswith(name), lib.ta_last_error()

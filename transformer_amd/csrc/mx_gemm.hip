@@ -71,7 +71,7 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const fl
 }
 
 // ---------------------------------------------------------------- few rows
-// A workgroup owns 16 NT rows of the weights (with GLU 8 NT gates and their ups) and all rows of x; its waves deal k out among
+// A workgroup owns 16 rows of the weights (with GLU 16 gates and their ups) and up to 16 rows of x; its waves deal k out among
 // them in chunks of 128 S and their sums meet in LDS in wave order. A load of the weights brings whole lines, eight blocks of
 // eight rows; the matrix instruction wants four blocks of sixteen, so the halves of every sixteen lanes trade places between the
 // loads of rows 0 to 7 and 8 to 15 (a move across lanes for each register, no LDS). x goes
@@ -83,49 +83,47 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const fl
 //
 // Waves: every CU wants some 16 of them with two chunks each on their way, which 64 KB of weights in flight keep the memory
 // busy with; fewer than four a workgroup leave too many of the sums' exchanges.
-template <bool X8, bool GLU, int MT, int NT, int S, int R>
-__global__ __launch_bounds__(MT > 1 ? 512 : 1024) void mx_few_kernel(MxGemm g, int bytes) {
-  static_assert(!GLU || NT % 2 == 0, "gates and ups");
-  static_assert(R <= 16 * MT && (S == 2 || S == 4), "rows of the tiles, loads in pairs");
+template <bool X8, bool GLU, int S, int R>
+__global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
+  if (gridDim.y > 1) {                          // this workgroup's R rows
+    const long long at = (long long)blockIdx.y * R;
+    g.x = (const unsigned char*)g.x + at * g.ldx * (X8 ? 1 : 2);
+    if (X8) g.xs += at * (g.K / MX_BLOCK);
+    g.out = (unsigned char*)g.out + at * g.ldo * (g.wide ? 4 : 2);
+    g.M = g.M - (int)at < R ? g.M - (int)at : R;
+  }
+  static_assert(R <= 16 && (S == 2 || S == 4), "rows of a tile, loads in pairs");
   constexpr int P = (X8 ? 8 : 16) * S;          // 16-byte pieces of a row of x in a chunk
   constexpr int FLIP = P < 16 ? P - 1 : 15;
-  constexpr int NO = GLU ? NT / 2 : NT;         // tiles of results
+  constexpr int NT = GLU ? 2 : 1;               // tiles of the weights
   constexpr int XI = R * P > 64 ? R * P / 64 : 1;               // loads of x
-  constexpr int LOADS = XI + NT * (S + 1) + (X8 ? MT : 0);      // of a chunk: at least so many
+  constexpr int LOADS = XI + NT * (S + 1) + (X8 ? 1 : 0);       // of a chunk: at least so many
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   // (what is the same in a whole wave is told to be: addresses are then one base and 32 bits a lane)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, q = lane / 16,
             waves = blockDim.x / 64;
-  const int n0 = blockIdx.x * 16 * NO, blocks = g.K / MX_BLOCK, chunks = blocks / (4 * S);
+  const int n0 = blockIdx.x * 16, blocks = g.K / MX_BLOCK, chunks = blocks / (4 * S);
   unsigned char* mine = mx_lds + wave * bytes;
-  const uint8_t *codes[GLU ? 2 : 1], *scales[GLU ? 2 : 1];      // of the workgroup's first row, of its first ups
+  const uint8_t *codes[NT], *scales[NT];        // of the workgroup's first row, of its first ups
 #pragma unroll
-  for (int u = 0; u < (GLU ? 2 : 1); ++u) {
-    codes[u] = g.codes + ((size_t)n0 + (u ? (size_t)g.N : 0)) * (g.K / 2);
-    scales[u] = g.scales + ((size_t)n0 + (u ? (size_t)g.N : 0)) * blocks;
+  for (int t = 0; t < NT; ++t) {
+    codes[t] = g.codes + ((size_t)n0 + (t ? (size_t)g.N : 0)) * (g.K / 2);
+    scales[t] = g.scales + ((size_t)n0 + (t ? (size_t)g.N : 0)) * blocks;
   }
-  uint32_t col[NO];                             // this lane's row of the weights, from n0 on
+  const uint32_t col = n0 + r < g.N ? r : g.N - 1 - n0;         // this lane's row of the weights, from n0 on
+  uint32_t piece_at[2];                         // what it loads: a block of row r % 8, of row 8 + r % 8
 #pragma unroll
-  for (int t = 0; t < NO; ++t) col[t] = n0 + 16 * t + r < g.N ? 16 * t + r : g.N - 1 - n0;
-  uint32_t piece_at[NO][2];                     // what this lane loads: a block of row r % 8, of row 8 + r % 8
-#pragma unroll
-  for (int t = 0; t < NO; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = 16 * t + 8 * h + r % 8;
-      piece_at[t][h] = (uint32_t)(n0 + at < g.N ? at : g.N - 1 - n0) * (uint32_t)(g.K / 2) + (q + 4 * (r / 8)) * 16;
-    }
-  uint32_t row[MT];                             // and of x
-#pragma unroll
-  for (int m = 0; m < MT; ++m) row[m] = 16 * m + r < g.M ? 16 * m + r : g.M - 1;
+  for (int h = 0; h < 2; ++h) {
+    const int at = 8 * h + r % 8;
+    piece_at[h] = (uint32_t)(n0 + at < g.N ? at : g.N - 1 - n0) * (uint32_t)(g.K / 2) + (q + 4 * (r / 8)) * 16;
+  }
+  const uint32_t row = r < g.M ? r : g.M - 1;   // and of x
   const uint32_t xstep = (uint32_t)g.ldx * (X8 ? 1 : 2);
-  mx_f32x4 acc[MT][NT];
+  mx_f32x4 acc[NT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[m][t] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NT; ++t) acc[t] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
   mx_u32x4 w[2][NT][S];
-  uint32_t ws[2][NT][S], xs[2][X8 ? MT : 1][S];
+  uint32_t ws[2][NT][S], xs[2][S];
 
   // all that chunk c needs, x first: it comes from a cache, and a wait that is too long by a few loads waits for it
   const auto ask = [&](int set, int c) {
@@ -137,16 +135,14 @@ __global__ __launch_bounds__(MT > 1 ? 512 : 1024) void mx_few_kernel(MxGemm g, i
       if (R * P >= 64 || at < R * P)
         ta_load_to_lds16((const unsigned char*)g.x + (size_t)c * P * 16, from * xstep + piece * 16, to + i * 1024);
     }
-    if (X8)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) __builtin_memcpy(xs[set][m], g.xs + (size_t)c * 4 * S + row[m] * (uint32_t)blocks, 4 * S);
+    if (X8) __builtin_memcpy(xs[set], g.xs + (size_t)c * 4 * S + row * (uint32_t)blocks, 4 * S);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      __builtin_memcpy(ws[set][t], scales[t / NO] + (size_t)c * 4 * S + col[t % NO] * (uint32_t)blocks, 4 * S);
+      __builtin_memcpy(ws[set][t], scales[t] + (size_t)c * 4 * S + col * (uint32_t)blocks, 4 * S);
 #pragma unroll
       for (int s = 0; s < S; ++s)
         w[set][t][s] = __builtin_nontemporal_load(
-            reinterpret_cast<const mx_u32x4*>(codes[t / NO] + (size_t)(c * S + s / 2 * 2) * 64 + piece_at[t % NO][s % 2]));
+            reinterpret_cast<const mx_u32x4*>(codes[t] + (size_t)(c * S + s / 2 * 2) * 64 + piece_at[s % 2]));
     }
   };
   // loads 2 i and 2 i + 1 to operands of steps 2 i and 2 i + 1: lanes 8 to 15 of the first take the second's of lanes 0 to 7,
@@ -165,50 +161,32 @@ __global__ __launch_bounds__(MT > 1 ? 512 : 1024) void mx_few_kernel(MxGemm g, i
   };
   const auto multiply = [&](int set) {
     const unsigned char* xl = mine + (size_t)set * R * P * 16;
-    const auto piece = [&](int m, int p) {
-      return *reinterpret_cast<const mx_u32x4*>(xl + ((size_t)row[m] * P + (p ^ (row[m] & FLIP))) * 16);
+    const auto piece = [&](int p) {
+      return *reinterpret_cast<const mx_u32x4*>(xl + (row * P + (p ^ (row & FLIP))) * 16);
     };
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       if (X8) {
         // lane group q holds the halves q % 2 of the 128 k's blocks q / 2 and 2 + q / 2, and block q's scale
-        mx_i32x8 a[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const mx_u32x4 lo = piece(m, 8 * s + q), hi = piece(m, 8 * s + 4 + q);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            a[m][i] = (int)lo[i];
-            a[m][4 + i] = (int)hi[i];
-          }
-        }
+        const mx_u32x4 lo = piece(8 * s + q), hi = piece(8 * s + 4 + q);
+        const mx_i32x8 a = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const mx_u32x4 c = w[set][t][s];
           const mx_i32x8 b = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            acc[m][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[m], b, acc[m][t], 0, 4, 0, (int)(xs[set][m][s] >> (8 * q)), 0,
-                                                                         (int)(ws[set][t][s] >> (8 * q)));
+          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], 0, 4, 0, (int)(xs[set][s] >> (8 * q)), 0,
+                                                                    (int)(ws[set][t][s] >> (8 * q)));
         }
       } else {
-        union {
-          mx_u32x4 u;
-          mx_bf16x8 v;
-        } a[MT][4];
+        mx_bf16x8 a[4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) a[m][j].u = piece(m, 16 * s + 4 * q + j);
+        for (int j = 0; j < 4; ++j) a[j] = __builtin_bit_cast(mx_bf16x8, piece(16 * s + 4 * q + j));
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const float scale = mx_scale(ws[set][t][s] >> (8 * q) & 255u);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const mx_bf16x8 b = mx_widen8(w[set][t][s][j], scale);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m][j].v, b, acc[m][t], 0, 0, 0);
-          }
+          for (int j = 0; j < 4; ++j)
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j], mx_widen8(w[set][t][s][j], scale), acc[t], 0, 0, 0);
         }
       }
     }
@@ -260,13 +238,11 @@ __global__ __launch_bounds__(MT > 1 ? 512 : 1024) void mx_few_kernel(MxGemm g, i
         w[0][t][s] = mx_u32x4{0, 0, 0, 0};
         ws[0][t][s] = 0x7f7f7f7fu;
         if (live) {
-          w[0][t][s] = *reinterpret_cast<const mx_u32x4*>(codes[t / NO] + (size_t)b * 16 + col[t % NO] * (uint32_t)(g.K / 2));
-          ws[0][t][s] = (uint32_t)scales[t / NO][b + col[t % NO] * (uint32_t)blocks] * 0x01010101u;
+          w[0][t][s] = *reinterpret_cast<const mx_u32x4*>(codes[t] + (size_t)b * 16 + col * (uint32_t)(g.K / 2));
+          ws[0][t][s] = (uint32_t)scales[t][b + col * (uint32_t)blocks] * 0x01010101u;
         }
       }
-      if (X8)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) xs[0][m][s] = live ? (uint32_t)g.xs[b + row[m] * (uint32_t)blocks] * 0x01010101u : 0x7f7f7f7fu;
+      if (X8) xs[0][s] = live ? (uint32_t)g.xs[b + row * (uint32_t)blocks] * 0x01010101u : 0x7f7f7f7fu;
     }
     multiply(0);
   }
@@ -274,24 +250,21 @@ __global__ __launch_bounds__(MT > 1 ? 512 : 1024) void mx_few_kernel(MxGemm g, i
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   float* part = reinterpret_cast<float*>(mine);
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[(m * NT + t) * 256 + (q * 4 + i) * 16 + r] = acc[m][t][i];
+    for (int i = 0; i < 4; ++i) part[t * 256 + (q * 4 + i) * 16 + r] = acc[t][i];
   __syncthreads();
-  for (int o = threadIdx.x; o < MT * NO * 256; o += blockDim.x) {
-    const int mt = o / (NO * 256), t = o / 256 % NO, at = o % 256;
-    const int m = 16 * mt + at / 16, n = n0 + 16 * t + at % 16;
+  for (int at = threadIdx.x; at < 256; at += blockDim.x) {
+    const int m = at / 16, n = n0 + at % 16;
     if (m >= g.M || n >= g.N) continue;
-    float v[2] = {0.f, 0.f};
+    float v[NT];
 #pragma unroll
-    for (int u = 0; u < (GLU ? 2 : 1); ++u) {
-      const int tile = (mt * NT + t + u * NO) * 256 + at;
-      for (int wv = 0; wv < waves; ++wv) v[u] += reinterpret_cast<const float*>(mx_lds + wv * bytes)[tile];
-      if (g.bias) v[u] += g.bias[n + (long long)u * g.N];
+    for (int t = 0; t < NT; ++t) {
+      v[t] = 0.f;
+      for (int wv = 0; wv < waves; ++wv) v[t] += reinterpret_cast<const float*>(mx_lds + wv * bytes)[t * 256 + at];
+      if (g.bias) v[t] += g.bias[n + (long long)t * g.N];
     }
-    const float y = GLU ? v[0] / (1.0f + expf(-v[0])) * v[1] : v[0];
+    const float y = GLU ? v[0] / (1.0f + expf(-v[0])) * v[NT - 1] : v[0];
     const long long to = (long long)m * g.ldo + n;
     if (g.wide) reinterpret_cast<float*>(g.out)[to] = y;
     else reinterpret_cast<bf16_t*>(g.out)[to] = from_f32<bf16_t>(y);
@@ -299,15 +272,14 @@ __global__ __launch_bounds__(MT > 1 ? 512 : 1024) void mx_few_kernel(MxGemm g, i
 }
 
 #define MX_LDS (160 * 1024)
-template <bool X8, bool GLU, int MT, int NT, int S, int R>
+template <bool X8, bool GLU, int S, int R>
 static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) {
-  constexpr int P = (X8 ? 8 : 16) * S, MOST = MT > 1 ? 8 : 16, NO = GLU ? NT / 2 : NT;
-  constexpr int x = R * P * 16, sums = MT * NT * 1024;
-  const auto kernel = mx_few_kernel<X8, GLU, MT, NT, S, R>;
-  const int chunks = g.K / (128 * S), grid = (g.N + NO * 16 - 1) / (NO * 16);
+  constexpr int x = R * (X8 ? 8 : 16) * S * 16, sums = (GLU ? 2 : 1) * 1024;
+  const auto kernel = mx_few_kernel<X8, GLU, S, R>;
+  const int chunks = g.K / (128 * S), grid = (g.N + 15) / 16;
   // as many waves as give every CU 16, then the fewest that need as many turns; one buffer of x does for one turn
   int waves = (16 * 256 + grid - 1) / grid;
-  waves = waves < 4 ? 4 : waves > MOST ? MOST : waves;
+  waves = waves < 4 ? 4 : waves > 16 ? 16 : waves;
   if (waves > chunks) waves = chunks > 0 ? chunks : 1;
   int bytes = waves < chunks ? 2 * x : x;
   if (bytes < sums) bytes = sums;
@@ -324,7 +296,7 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
     if (e != hipSuccess) return ta_fail("%s: %d bytes of LDS refused (%s)", what, MX_LDS, hipGetErrorString(e));
     allowed = MX_LDS;
   }
-  kernel<<<grid, waves * 64, (size_t)waves * bytes, stream>>>(g, bytes);
+  kernel<<<dim3(grid, (g.M + R - 1) / R), waves * 64, (size_t)waves * bytes, stream>>>(g, bytes);
   return ta_check_launch(what);
 }
 
@@ -813,15 +785,20 @@ static int mx_gemm_check(const char* what, const MxGemm& g) {
   return 0;
 }
 
-// Rows up to which the waves along k have it, by GPU time against the tiles'.
-static bool mx_few(bool x8, bool glu, int M, int N, int K) {
-  (void)x8; (void)glu; (void)N; (void)K;
-  return M <= 16;
+// Whether the waves along k take it: up to 16 rows always; more in groups of 16, each of which reads the weights again, where that
+// is less than what the tiles cost (GPU time in us: 2.3 + 0.24, with 8 bits 0.20, for every million weights and group against the
+// tiles' steps, planes and scales and 7; 32 rows of 4,096 over k = 4,096 10 against 14, over 14,336 30 against 21).
+static bool mx_few(bool x8, bool glu, int M, int N, int K, bool aligned) {
+  if (M <= 16) return true;
+  if (M > 64) return false;
+  const MxPlan plan = mx_plan(x8, glu, M, N, K, aligned);
+  const double weights = (double)N * (glu ? 2 : 1) * K * 1e-6;
+  return 2.3 + (M + 15) / 16 * weights * (x8 ? 0.20 : 0.24) < plan.us + 7. + (plan.scales ? 2.5 : 0.);
 }
 
 // Bytes of scratch for M rows in 8 bits (x8) or bfloat16; aligned: all scales start on 16 bytes.
 extern "C" long long ta_gemm_mx4_scratch(int x8, int swiglu, int M, int N, int K, int aligned) {
-  if (M <= 0 || N <= 0 || K < MX_BLOCK || mx_few(x8, swiglu, M, N, K)) return 0;
+  if (M <= 0 || N <= 0 || K < MX_BLOCK || mx_few(x8, swiglu, M, N, K, aligned)) return 0;
   return mx_plan(x8, swiglu, M, N, K, aligned).bytes;
 }
 
@@ -840,18 +817,18 @@ extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const 
   TA_REQUIRE(ldx <= 1 << 24 && K <= 1 << 23, "%s: rows %lld apart, k %d: at most 16,777,216 and 8,388,608", what, ldx, K);   // a tile's rows within 32 bits
   TA_REQUIRE(!swiglu || N <= 0x3fffffff, "%s: %d gates", what, N);
   if (M == 0) return 0;
-  if (!mx_few(false, swiglu, M, N, K))
+  if (!mx_few(false, swiglu, M, N, K, (uintptr_t)scales % 16 == 0))
     return swiglu ? mx_tiles<false, true>(what, stream, g, scratch, scratch_bytes) : mx_tiles<false, false>(what, stream, g, scratch, scratch_bytes);
   if (swiglu) {
-    if (M <= 1) return mx_few_launch<false, true, 1, 2, 2, 1>(what, stream, g);
-    if (M <= 4) return mx_few_launch<false, true, 1, 2, 2, 4>(what, stream, g);
-    if (M <= 8) return mx_few_launch<false, true, 1, 2, 2, 8>(what, stream, g);
-    return mx_few_launch<false, true, 1, 2, 2, 16>(what, stream, g);
+    if (M <= 1) return mx_few_launch<false, true, 2, 1>(what, stream, g);
+    if (M <= 4) return mx_few_launch<false, true, 2, 4>(what, stream, g);
+    if (M <= 8) return mx_few_launch<false, true, 2, 8>(what, stream, g);
+    return mx_few_launch<false, true, 2, 16>(what, stream, g);
   }
-  if (M <= 1) return mx_few_launch<false, false, 1, 1, 4, 1>(what, stream, g);
-  if (M <= 4) return mx_few_launch<false, false, 1, 1, 4, 4>(what, stream, g);
-  if (M <= 8) return mx_few_launch<false, false, 1, 1, 4, 8>(what, stream, g);
-  return mx_few_launch<false, false, 1, 1, 2, 16>(what, stream, g);
+  if (M <= 1) return mx_few_launch<false, false, 4, 1>(what, stream, g);
+  if (M <= 4) return mx_few_launch<false, false, 4, 4>(what, stream, g);
+  if (M <= 8) return mx_few_launch<false, false, 4, 8>(what, stream, g);
+  return mx_few_launch<false, false, 2, 16>(what, stream, g);
 }
 
 // 8-bit rows, codes [M][K] and bytes [M][K/32]; out bfloat16. scratch: ta_gemm_mx4_scratch bytes on 16.
@@ -862,9 +839,9 @@ extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs
   if (mx_gemm_check(what, g)) return 1;
   TA_REQUIRE(K <= 1 << 23, "%s: k %d: at most 8,388,608", what, K);         // 256 rows within 31 bits
   if (M == 0) return 0;
-  if (!mx_few(true, false, M, N, K)) return mx_tiles<true, false>(what, stream, g, scratch, scratch_bytes);
-  if (M <= 1) return mx_few_launch<true, false, 1, 1, 4, 1>(what, stream, g);
-  if (M <= 4) return mx_few_launch<true, false, 1, 1, 4, 4>(what, stream, g);
-  if (M <= 8) return mx_few_launch<true, false, 1, 1, 4, 8>(what, stream, g);
-  return mx_few_launch<true, false, 1, 1, 4, 16>(what, stream, g);
+  if (!mx_few(true, false, M, N, K, ((uintptr_t)xs | (uintptr_t)scales) % 16 == 0)) return mx_tiles<true, false>(what, stream, g, scratch, scratch_bytes);
+  if (M <= 1) return mx_few_launch<true, false, 4, 1>(what, stream, g);
+  if (M <= 4) return mx_few_launch<true, false, 4, 4>(what, stream, g);
+  if (M <= 8) return mx_few_launch<true, false, 2, 8>(what, stream, g);
+  return mx_few_launch<true, false, 2, 16>(what, stream, g);
 }
