@@ -62,7 +62,6 @@ def test_rows_refuse_what_their_kernels_do_not_take():
     for d, ld, p, bias, dtype in ((48, 96, AT, None, 0), (64, 124, AT, None, 0), (64, 130, AT, None, 0), (64, 132, AT, None, 1), (64, 128, off, None, 0),
                                   (64, 128, AT, off, 0), (64, 128, AT, None, 2)):
         _refused(lib.ta_swiglu_mx8(None, c_int(dtype), p, ll(ld), bias, AT, AT, ll(3), c_int(d)), b"ta_swiglu_mx8")
-    _refused(lib.ta_mx8_pack(None, c_int(0), AT, ll(1 << 20), AT, AT, ll(1 << 40), c_int(1 << 20)), b"ta_mx8_pack")
 
     def norm(n=3, d=64, planes=0, delta=None, to=AT, bias=None, x=AT, dtype=0):
         return lib.ta_add_rmsnorm_mx8(None, c_int(dtype), x, delta, c_int(planes), bias, AT, c_float(1e-5), to, AT, AT, c_int(n), c_int(d))
