@@ -9,7 +9,6 @@
 // of magnitudes where the operands' exponents fill their range); results are therefore bfloat16, which rounds 80 times as
 // coarsely, and only the running sums over k are float32.
 #include "mx.h"
-#include <type_traits>
 
 __device__ __forceinline__ mx_bf16x8 mx_widen8(uint32_t codes, float scale) {
   union {
@@ -314,7 +313,7 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
 //
 // The weights are the first operand: a lane then holds 4 neighbouring columns of one row. Row p of the tile t of 16 stands for
 // column 16 (p / 4) + 4 t + p % 4 of the wave's 64, so a lane's four tiles are 16 neighbouring columns, stored 16 bytes at a time.
-// Pieces of 16 bytes are permuted by the row's number, so that eight lanes' reads meet no bank twice.
+// Pieces of 16 bytes are permuted by the row's number, so that sixteen lanes' reads meet no bank twice.
 // Where the tiles do not fill the CUs, k is cut among `parts` workgroups, which leave float32 sums in planes; mx_planes_kernel adds
 // them in order and finishes. GLU: a tile holds 64 gates and their 64 ups, a lane's 16 columns are then 8 of either.
 struct MxTiles {
@@ -330,10 +329,17 @@ __device__ __forceinline__ void mx_to_lds16(const void* base, uint32_t offset, u
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "m0", "memory");
 }
 
+// which of a row's pieces lie where: sixteen rows' reads of a piece meet every bank once, two rows of 8 pieces (of 256 bytes
+// together) or one of 16 in each of the places that a bank has
+template <bool X8>
+__device__ __forceinline__ uint32_t mx_flip(uint32_t row) {
+  return X8 ? row >> 1 & 7 : row & 15;
+}
+
 template <bool X8, bool GLU, int BM, int BN, int WM, int WN, int KG, int NS>
 __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   constexpr int W = 8, TM = BM / (16 * WM), XB = X8 ? 128 : 256;        // bytes of a row of x in a step
-  constexpr int XP = XB / 16, FLIP = X8 ? 7 : 15;                       // its pieces
+  constexpr int XP = XB / 16;                                           // its pieces
   constexpr int XL = BM * XB / 1024 / W, WL = BN / 16 / W;     // loads of 1 KB a wave and step
   constexpr int SX = X8 ? BM : 0, SL = (SX + BN) / 64;         // loads of 64 rows' scales, one a wave
   constexpr int LOADS = XL + WL;
@@ -346,7 +352,10 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   // workgroups go round the 8 XCDs: each gets neighbouring tiles, all rows of a band of columns, so that its cache holds them
   const int tiles = z.m_tiles * z.n_tiles, per = tiles / 8, b = blockIdx.x % tiles, cut = blockIdx.x / tiles;
   const int tile = b < per * 8 ? (b % 8) * per + b / 8 : b;
-  const int m0 = tile % z.m_tiles * BM, n0 = tile / z.m_tiles * (GLU ? BN / 2 : BN);
+  // bands of four tiles of rows, columns after columns inside a band: the 32 tiles that an XCD has under way then read a quarter of
+  // the rows and eight columns' weights and not all rows
+  const int band = tile / (4 * z.n_tiles), in = tile % (4 * z.n_tiles), high = z.m_tiles - 4 * band < 4 ? z.m_tiles - 4 * band : 4;
+  const int m0 = (4 * band + in % high) * BM, n0 = in / high * (GLU ? BN / 2 : BN);
   const int first = cut * z.part_steps, left = (g.K + 127) / 128 - first;       // this part's steps
   const int steps = left < z.part_steps ? left : z.part_steps;
   const int whole_steps = g.K / 128 - first, full = whole_steps < steps ? whole_steps : steps;
@@ -357,7 +366,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   uint32_t xo[XL], wo[WL], so;
 #pragma unroll
   for (int i = 0; i < XL; ++i) {
-    const int at = (wave * XL + i) * 64 + lane, row = at / XP, piece = (at % XP) ^ (row & FLIP);
+    const int at = (wave * XL + i) * 64 + lane, row = at / XP, piece = (at % XP) ^ mx_flip<X8>(row);
     xo[i] = (uint32_t)(m0 + row < g.M ? row : g.M - 1 - m0) * ((uint32_t)g.ldx * (X8 ? 1 : 2)) + piece * 16;
   }
   // row of the weights, from n0 on, behind row `row` of the tile
@@ -374,29 +383,43 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   const int sl = wave % SL;                     // waves beyond the scales' loads bring some of them once more
   const bool s_x = sl < SX / 64;
   {
-    const int row = (s_x ? sl : sl - SX / 64) * 64 + lane;
+    // (16-byte places: of every 64 rows' scales, those that a wave reads at once, 16 apart, lie in different banks)
+    const int row = (s_x ? sl : sl - SX / 64) * 64 + (lane ^ (lane >> 4 & 3) * 4);
     so = (s_x ? (uint32_t)(m0 + row < g.M ? row : g.M - 1 - m0) : weight_row(row)) * (uint32_t)z.step;
   }
   const unsigned char* sbase = (s_x ? z.xs + (size_t)m0 * z.step : z.ws + (size_t)n0 * z.step) + (size_t)first * 4;
 
   uint32_t to_lds = 0;                          // the place of the next step asked for
   const unsigned char *xk = x, *wk = w, *sk = sbase;
-  // BULK: a whole step; else one that k may end inside of, or none any more
-  const auto ask = [&](auto bulk, int step) {
-    constexpr bool BULK = decltype(bulk)::value;
-    if (!BULK && step >= steps) return;
-    // scales first, so that a wait that counts the operands alone waits for no more than them
-    if (step % 4 == 0) mx_to_lds16(sk, so, AT_S + (step & 4) / 4 * GROUP + sl * 1024);
-    if (BULK || step < full) {
+  // a whole step's loads, one by one: scales first, so that a wait that counts the operands alone waits for no more than them
+  const auto ask_one = [&](int step, int i) {
+    if (i == 0 && step % 4 == 0) mx_to_lds16(sk, so, AT_S + (step & 4) / 4 * GROUP + sl * 1024);
+    if (i < XL) mx_to_lds16(xk, xo[i < XL ? i : 0], to_lds + (wave * XL + i) * 1024);
+    else mx_to_lds16(wk, wo[i >= XL ? i - XL : 0], to_lds + AT_W + (wave * WL + i - XL) * 1024);
+  };
+  const auto asked = [&]() {
+    xk += XB;
+    wk += 64;
+    sk += 4;
+    to_lds = to_lds == (NS - 1) * STAGE ? 0 : to_lds + STAGE;
+  };
+  const auto ask_all = [&](int step) {
 #pragma unroll
-      for (int i = 0; i < XL; ++i) mx_to_lds16(xk, xo[i], to_lds + (wave * XL + i) * 1024);
-#pragma unroll
-      for (int i = 0; i < WL; ++i) mx_to_lds16(wk, wo[i], to_lds + AT_W + (wave * WL + i) * 1024);
+    for (int i = 0; i < LOADS; ++i) ask_one(step, i);
+    asked();
+  };
+  // a step that k may end inside of, or none any more
+  const auto ask = [&](int step) {
+    if (step >= steps) return;
+    if (step < full) {
+      ask_all(step);
+      return;
     } else {
       // k ends inside this step: nothing behind it, zero in x, any codes in w
+      if (step % 4 == 0) mx_to_lds16(sk, so, AT_S + (step & 4) / 4 * GROUP + sl * 1024);
 #pragma unroll
       for (int i = 0; i < XL; ++i) {
-        const int at = (wave * XL + i) * 64 + lane, row = at / XP, piece = (at % XP) ^ (row & FLIP);
+        const int at = (wave * XL + i) * 64 + lane, row = at / XP, piece = (at % XP) ^ mx_flip<X8>(row);
         if (step * XP + piece < pieces) mx_to_lds16(xk, xo[i], to_lds + (wave * XL + i) * 1024);
         else reinterpret_cast<mx_u32x4*>(mx_lds + to_lds + (wave * XL + i) * 1024)[lane] = mx_u32x4{0, 0, 0, 0};
       }
@@ -406,10 +429,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
         if (step * 4 + piece < wpieces) mx_to_lds16(wk, wo[i], to_lds + AT_W + (wave * WL + i) * 1024);
       }
     }
-    xk += XB;
-    wk += 64;
-    sk += 4;
-    to_lds = to_lds == (NS - 1) * STAGE ? 0 : to_lds + STAGE;
+    asked();
   };
 
   mx_f32x4 acc[TM][4];
@@ -425,17 +445,17 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   // where a lane reads: the tiles lie a fixed number of bytes apart
   const uint32_t w_at = AT_W + (wn * 64 + 16 * (r / 4) + r % 4) * 64 + (q ^ (r / 4)) * 16;
   const uint32_t x_at = (wm * TM * 16 + r) * XB;
-  const uint32_t ws_at = AT_S + (SX + wn * 64 + 16 * (r / 4) + r % 4) * 16 + q, xs_at = AT_S + (wm * TM * 16 + r) * 16 + q;
+  const uint32_t ws_at = AT_S + (SX + wn * 64 + 16 * (r / 4) + r % 4) * 16 + q, xs_at = AT_S + wm * TM * 256 + q;
   uint32_t from = KG == 2 && group ? STAGE : 0;  // the place of the step to read
   const unsigned char *xl, *xsl;
   const auto read_x = [&](int m) {
 #pragma unroll
     for (int i = 0; i < XP / 4; ++i) {
       // 8 bits: halves q % 2 of the blocks q / 2 and 2 + q / 2; bfloat16: the four eights of block q
-      const uint32_t piece = X8 ? (uint32_t)(q + 4 * i) ^ (r & FLIP) : (uint32_t)(4 * q + i) ^ (r & FLIP);
+      const uint32_t piece = X8 ? (uint32_t)(q + 4 * i) ^ mx_flip<X8>(r) : (uint32_t)(4 * q + i) ^ mx_flip<X8>(r);
       xf[m % HELD][i] = *reinterpret_cast<const mx_u32x4*>(xl + piece * 16 + m * 16 * XB);
     }
-    if (X8) xs[m % HELD] = xsl[m * 256];
+    if (X8) xs[m % HELD] = xsl[m * 256 + (r ^ ((wm * TM + m) & 3) * 4) * 16];
   };
   const auto read = [&](int step) {
     const uint32_t sc = (step & 4) / 4 * GROUP + (step & 3) * 4;
@@ -445,14 +465,25 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       wf[t] = *reinterpret_cast<const mx_u32x4*>(wl + t * 256);
-      ws[t] = wsl[t * 64];
+      ws[t] = wsl[(t ^ r / 4) * 64];
     }
 #pragma unroll
     for (int m = 0; m < HELD; ++m) read_x(m);
     from += KG * STAGE;
     from = from >= NS * STAGE ? from - NS * STAGE : from;
   };
-  const auto multiply = [&]() {
+  // `step`: a whole step whose loads go out between the products (-1: none), where a phase has many: in front of them they keep a wave for
+  // as long as the cache takes to accept them (512 x 28,672 x 4,096 58 us so, 55 between; in the small tiles of KG 2 they go out first,
+  // 26 and 29 us of 64 rows of bfloat16 against 2 x 14,336 x 4,096: there the way to memory is what a phase waits for)
+  const auto multiply = [&](int step) {
+    const auto between = [&](int i, int count) {
+      if (step >= 0) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+          if (j * count / LOADS == i) ask_one(step, j);
+      }
+      if (KG == 1) __builtin_amdgcn_sched_barrier(0);
+    };
     if constexpr (X8) {
 #pragma unroll
       for (int m = 0; m < TM; ++m) {
@@ -463,7 +494,9 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
           const mx_i32x8 a = {(int)wf[t][0], (int)wf[t][1], (int)wf[t][2], (int)wf[t][3], 0, 0, 0, 0};
           acc[m][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, v, acc[m][t], 4, 0, 0, ws[t], 0, xs[m % HELD]);
         }
-        if (m + HELD < TM) read_x(m + HELD);
+        if (KG == 1) __builtin_amdgcn_sched_barrier(0);
+        if (m + HELD < TM) read_x(m + HELD);     // here: the compiler would put it right in front of its use
+        between(m, TM);
       }
     } else {
 #pragma unroll
@@ -478,6 +511,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
         }
       }
     }
+    if (step >= 0) asked();
   };
   // the end of a phase; `next`: the step that has to be there then (none: -1), with whole steps up to `asked` asked for behind it
   const auto end = [&](int next, int asked) {
@@ -497,11 +531,8 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  const std::integral_constant<bool, true> inside{};
-  const std::integral_constant<bool, false> any{};
-
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) ask(any, i);
+  for (int i = 0; i < NS - 1; ++i) ask(i);
   end(0, NS - 2);
   if (KG == 1) {
     // phases 2 k and 2 k + 1: group 0 reads step k, then multiplies; group 1 multiplies step k - 1, then reads step k; in the
@@ -510,32 +541,31 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
     if (group) {
       end(-1, 0);
       for (; k + NS <= full; ++k) {
-        ask(inside, k + NS - 1);
         read(k);
+        ask_all(k + NS - 1);
         end_inside(true);
-        multiply();
+        multiply(-1);
         end_inside(false);
       }
       for (; k < steps; ++k) {
-        ask(any, k + NS - 1);
         read(k);
+        ask(k + NS - 1);
         end(k + 1, k + NS - 1);
-        multiply();
+        multiply(-1);
         end(-1, 0);
       }
     } else {
       for (; k + NS <= full; ++k) {
         read(k);
         end_inside(false);
-        ask(inside, k + NS - 1);
-        multiply();
+        multiply(k + NS - 1);
         end_inside(true);
       }
       for (; k < steps; ++k) {
         read(k);
         end(-1, 0);
-        ask(any, k + NS - 1);
-        multiply();
+        ask(k + NS - 1);
+        multiply(-1);
         end(k + 1, k + NS - 1);
       }
       end(-1, 0);
@@ -544,24 +574,24 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
     // phase p: the group p % 2 reads step p, the other multiplies step p - 1, both ask
     int p = 0;
     if (group) {
-      ask(any, NS - 1);
+      ask(NS - 1);
       end(1, NS - 1);
       p = 1;
     }
     for (; p + NS + 1 <= full; p += 2) {
-      ask(inside, p + NS - 1);
+      ask_all(p + NS - 1);
       read(p);
       end_inside(true);
-      ask(inside, p + NS);
-      multiply();
+      ask_all(p + NS);
+      multiply(-1);
       end_inside(true);
     }
     for (; p < steps; p += 2) {
-      ask(any, p + NS - 1);
       read(p);
+      ask(p + NS - 1);
       end(p + 1, p + NS - 1);
-      ask(any, p + NS);
-      multiply();
+      ask(p + NS);
+      multiply(-1);
       end(p + 2, p + NS);
     }
     if (p == steps) end(-1, 0);                  // as many phases for either group: the last of them was the other's
