@@ -316,12 +316,13 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
 // Pieces of 16 bytes are permuted by the row's number, so that sixteen lanes' reads meet no bank twice.
 // Where the tiles do not fill the CUs, k is cut among `parts` workgroups, which leave float32 sums in planes; mx_planes_kernel adds
 // them in order and finishes. GLU: a tile holds 64 gates and their 64 ups, a lane's 16 columns are then 8 of either.
+__device__ __host__ __forceinline__ long long mx_pad(int n) { return (n + 3LL) / 4 * 4; }
 struct MxTiles {
   const uint8_t *xs, *ws;     // scales in rows of `step` bytes, a multiple of 16, 127 behind the last block
   int step;
   int m_tiles, n_tiles;
   int parts, part_steps;      // steps of a part, a multiple of 4
-  float* planes;              // [parts][M][rows of the weights], or null
+  float* planes;              // [parts][M][mx_pad(N), with GLU twice], or null
 };
 
 // 16 bytes a lane to the LDS that starts at `lds`; base and lds are the whole wave's
@@ -618,7 +619,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
 
   if (z.planes) {
     // rows of the weights in this lane's registers: 4 t + i behind the first, with GLU 8 gates and 8 ups
-    const long long rows = GLU ? 2LL * g.N : g.N;
+    const long long rows = (GLU ? 2 : 1) * mx_pad(g.N);
     const int n = n0 + (GLU ? wn * 32 + 8 * q : wn * 64 + 16 * q);
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
@@ -628,29 +629,28 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int c = GLU ? 4 * (t % 2) : 4 * t;
-        float* to = o + c + (GLU && t >= 2 ? g.N : 0);
-        if (n + c + 4 <= g.N && rows % 4 == 0 && (!GLU || g.N % 4 == 0)) *reinterpret_cast<mx_f32x4*>(to) = acc[m][t];
-        else
-          for (int i = 0; i < 4; ++i)
-            if (n + c + i < g.N) to[i] = acc[m][t][i];
+        if (n + c < g.N) *reinterpret_cast<mx_f32x4*>(o + c + (GLU && t >= 2 ? mx_pad(g.N) : 0)) = acc[m][t];
       }
     }
     return;
   }
   constexpr int CN = GLU ? 8 : 16;               // this lane's columns of the result
-  const int n = n0 + wn * (4 * CN) + CN * q;
+  const int n_wave = n0 + wn * (4 * CN), n = n_wave + CN * q;
   float add[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int c = i % CN;
     add[i] = g.bias && n + c < g.N ? g.bias[n + c + (i >= CN ? (long long)g.N : 0)] : 0.f;
   }
-  const int piece = g.wide ? 4 : 8;
-  const bool whole = n + CN <= g.N && g.ldo % piece == 0 && (uintptr_t)g.out % 16 == 0;
+  const bool pieces16 = g.ldo % (g.wide ? 4 : 8) == 0 && (uintptr_t)g.out % 16 == 0;
+  // rows that do not start on 16 bytes go through LDS (the wave's own, as far as it has just read it alone) and out a row at a time:
+  // single columns straight from the registers would be 64 places in memory a store (1,638 x 2,518 over k = 704 29 us)
+  constexpr int PAD = 4 * CN + 4;
+  float* mine = reinterpret_cast<float*>(mx_lds + part * (KG == 2 ? TM * 4096 : 16 * PAD * 4));
+  static_assert(16 * PAD * 4 <= (KG == 2 ? TM * 4096 : STAGE), "a wave's tile of results");
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
-    const int row = m0 + (wm * TM + m) * 16 + r;
-    if (row >= g.M) continue;
+    const int row0 = m0 + (wm * TM + m) * 16, row = row0 + r;
     float y[CN];
 #pragma unroll
     for (int i = 0; i < CN; ++i) {
@@ -662,7 +662,25 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
         y[i] = v;
       }
     }
-    mx_store<CN>(g, (long long)row * g.ldo + n, y, whole, g.N - n);
+    if (pieces16) {
+      if (row < g.M) mx_store<CN>(g, (long long)row * g.ldo + n, y, n + CN <= g.N, g.N - n);
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < CN; i += 4)
+      *reinterpret_cast<mx_f32x4*>(mine + r * PAD + CN * q + i) = mx_f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i += 16 / CN) {
+      const int at = i + lane / (4 * CN), c = lane % (4 * CN);
+      if (row0 + at < g.M && n_wave + c < g.N) {
+        const long long to = (long long)(row0 + at) * g.ldo + n_wave + c;
+        const float v = mine[at * PAD + c];
+        if (g.wide) reinterpret_cast<float*>(g.out)[to] = v;
+        else reinterpret_cast<bf16_t*>(g.out)[to] = from_f32<bf16_t>(v);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // read before the next tile overwrites it
   }
 }
 
@@ -673,27 +691,15 @@ __global__ __launch_bounds__(256) void mx_planes_kernel(MxGemm g, const float* _
   const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
   const int row = (int)(at / per), n = (int)(at % per) * 4;
   if (row >= g.M) return;
-  const long long rows = GLU ? 2LL * g.N : g.N, plane = (long long)g.M * rows;
-  const bool four = n + 4 <= g.N && g.N % 4 == 0;
+  const long long pad = mx_pad(g.N), rows = (GLU ? 2 : 1) * pad, plane = g.M * rows;
   float v[2][4];
 #pragma unroll
   for (int u = 0; u < (GLU ? 2 : 1); ++u) {
-    const float* p = planes + row * rows + n + (u ? g.N : 0);
+    const float* p = planes + row * rows + n + u * pad;
+    mx_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < parts; ++c, p += plane) sum += *reinterpret_cast<const mx_f32x4*>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[u][i] = 0.f;
-    for (int c = 0; c < parts; ++c, p += plane) {
-      if (four) {
-        const mx_f32x4 t = *reinterpret_cast<const mx_f32x4*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] += t[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] += n + i < g.N ? p[i] : 0.f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (g.bias && n + i < g.N) v[u][i] += g.bias[n + i + (u ? (long long)g.N : 0)];
+    for (int i = 0; i < 4; ++i) v[u][i] = sum[i] + (g.bias && n + i < g.N ? g.bias[n + i + (u ? (long long)g.N : 0)] : 0.f);
   }
   float y[4];
 #pragma unroll
@@ -764,7 +770,7 @@ static MxPlan mx_plan(bool x8, bool glu, int M, int N, int K, bool aligned) {
       // planes are written and read once at some 4 TB/s, by a kernel of their own
       const double planes = parts > 1 ? 2.5 + (double)parts * M * rows * 8 * 0.25e-6 : 0.;
       const double us = (double)((tiles * parts + 255) / 256) * (each < steps ? each : steps) * mx_forms[f].us * (x8 ? 1. : 1.3) + planes;
-      if (us < best.us) best = {f, parts, each, false, 0, parts > 1 ? parts * (long long)M * rows * 4 : 0, us};
+      if (us < best.us) best = {f, parts, each, false, 0, parts > 1 ? parts * (long long)M * (glu ? 2 : 1) * mx_pad(N) * 4 : 0, us};
     }
   }
   best.scales = K % 512 != 0 || !aligned;
