@@ -30,18 +30,17 @@ def test_products_refuse_what_their_kernels_do_not_take():
                dict(M=65), dict(N=1 << 30, glu=1), dict(ldx=(1 << 24) + 8), dict(K=(1 << 23) + 32)):
         _refused(_gemm(lib, **kw), b"ta_gemm_mx4:")
     for kw in (dict(K=48), dict(M=-1), dict(N=0), dict(x=off), dict(ldo=63), dict(M=2147483647, N=2147483647), dict(K=(1 << 23) + 32),
-               dict(M=65, K=96), dict(M=65, K=96, scratch=AT, room=(65 + 64) * 16 - 1), dict(M=65, K=96, scratch=c_void_p((1 << 20) + 8), room=1 << 20),
-               dict(M=65, K=512, xs=c_void_p((1 << 20) + 1))):
+               dict(M=12000, N=12000, K=2080), dict(M=12000, N=12000, K=2080, scratch=AT, room=24000 * 80 - 1),
+               dict(M=12000, N=12000, K=2080, scratch=c_void_p((1 << 20) + 8), room=1 << 30),
+               dict(M=12000, N=12000, K=2048, xs=c_void_p((1 << 20) + 1))):
         _refused(_gemm8(lib, **kw), b"ta_gemm_mx4_mx8:")
     assert lib.ta_mx4_max_rows() == kernels.MX4_MAX_ROWS
     # more rows: scratch for scales off 16 bytes, (rows of x in 8 bits and of the weights) * 16 bytes every 512 k, and for planes
+    for K, need in ((96, 0), (512, 0), (1024, 0), (2048, 0), (2080, 24000 * 80)):
+        assert kernels.gemm_mx4_scratch(True, False, 12000, 12000, K) == need
+    assert kernels.gemm_mx4_scratch(True, False, 12000, 12000, 2048, False) == 24000 * 64
     for eight in (False, True):
-        for glu in (False, True)[:1 if eight else 2]:
-            for M, N, K, need in ((kernels.MX_FEW_ROWS, 70, 96, 0), (200, 70, 96, ((200 if eight else 0) + (140 if glu else 70)) * 16), (200, 70, 512, 0)):
-                if eight:
-                    assert kernels.gemm_mx4_scratch(eight, glu, M, N, K) == need
-        if eight:
-            assert kernels.gemm_mx4_scratch(eight, False, 200, 64, 512, False) == 264 * 16
+        assert kernels.gemm_mx4_scratch(eight, False, kernels.MX_FEW_ROWS, 70, 96) == 0
         need = kernels.gemm_mx4_scratch(eight, False, 64, 4096, 14336)
         assert need and need % (64 * 4096 * 4) == 0
         call = _gemm8 if eight else _gemm

@@ -318,8 +318,8 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
 // them in order and finishes. GLU: a tile holds 64 gates and their 64 ups, a lane's 16 columns are then 8 of either.
 __device__ __host__ __forceinline__ long long mx_pad(int n) { return (n + 3LL) / 4 * 4; }
 struct MxTiles {
-  const uint8_t *xs, *ws;     // scales in rows of `step` bytes, a multiple of 16, 127 behind the last block
-  int step;
+  const uint8_t *xs, *ws;     // scales in rows of `step` bytes, a multiple of 16, 127 behind the last block; or, with a step of 0, as
+  int step;                   // they are, and a part has 8 steps at most: a tile's scales come in through registers in front of them
   int m_tiles, n_tiles;
   int parts, part_steps;      // steps of a part, a multiple of 4
   float* planes;              // [parts][M][mx_pad(N), with GLU twice], or null
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   const unsigned char *xk = x, *wk = w, *sk = sbase;
   // a whole step's loads, one by one: scales first, so that a wait that counts the operands alone waits for no more than them
   const auto ask_one = [&](int step, int i) {
-    if (i == 0 && step % 4 == 0) mx_to_lds16(sk, so, AT_S + (step & 4) / 4 * GROUP + sl * 1024);
+    if (i == 0 && step % 4 == 0 && z.step) mx_to_lds16(sk, so, AT_S + (step & 4) / 4 * GROUP + sl * 1024);
     if (i < XL) mx_to_lds16(xk, xo[i < XL ? i : 0], to_lds + (wave * XL + i) * 1024);
     else mx_to_lds16(wk, wo[i >= XL ? i - XL : 0], to_lds + AT_W + (wave * WL + i - XL) * 1024);
   };
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
       return;
     } else {
       // k ends inside this step: nothing behind it, zero in x, any codes in w
-      if (step % 4 == 0) mx_to_lds16(sk, so, AT_S + (step & 4) / 4 * GROUP + sl * 1024);
+      if (step % 4 == 0 && z.step) mx_to_lds16(sk, so, AT_S + (step & 4) / 4 * GROUP + sl * 1024);
 #pragma unroll
       for (int i = 0; i < XL; ++i) {
         const int at = (wave * XL + i) * 64 + lane, row = at / XP, piece = (at % XP) ^ mx_flip<X8>(row);
@@ -534,6 +534,23 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
   };
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) ask(i);
+  if (!z.step) {
+    const int blocks = g.K / MX_BLOCK;
+    for (int at = threadIdx.x; at < 2 * (SX + BN); at += 512) {
+      const int half = at / (SX + BN), place = at % (SX + BN), row = place < SX ? place : place - SX, b = first * 4 + half * 16;
+      const uint8_t* from = place < SX ? z.xs + (size_t)(m0 + row < g.M ? m0 + row : g.M - 1) * blocks
+                                       : z.ws + ((size_t)n0 + weight_row(row)) * blocks;
+      mx_u32x4 v = {0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+      if (b + 16 <= blocks) {
+        __builtin_memcpy(&v, from + b, 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (b + i < blocks) v[i / 4] = (v[i / 4] & ~(255u << (8 * (i % 4)))) | (uint32_t)from[b + i] << (8 * (i % 4));
+      }
+      *reinterpret_cast<mx_u32x4*>(mx_lds + AT_S + half * GROUP + (place ^ (place >> 4 & 3) * 4) * 16) = v;
+    }
+  }
   end(0, NS - 2);
   if (KG == 1) {
     // phases 2 k and 2 k + 1: group 0 reads step k, then multiplies; group 1 multiplies step k - 1, then reads step k; in the
@@ -760,6 +777,7 @@ static int mx_step(int K) { return (K + 511) / 512 * 16; }
 static MxPlan mx_plan(bool x8, bool glu, int M, int N, int K, bool aligned) {
   const long long rows = glu ? 2LL * N : N;
   const int steps = (K + 127) / 128;
+  const bool odd = K % 512 != 0 || !aligned;     // scales whose rows do not start on 16 bytes: laid out again, but where a part has few steps
   MxPlan best = {};
   best.us = 1e30;
   for (int f = 0; f < (x8 ? 4 : 1); ++f) {
@@ -769,11 +787,12 @@ static MxPlan mx_plan(bool x8, bool glu, int M, int N, int K, bool aligned) {
       if (parts > 1 && (tiles * parts > 512 || (long long)(parts - 1) * each >= steps)) break;
       // planes are written and read once at some 4 TB/s, by a kernel of their own
       const double planes = parts > 1 ? 2.5 + (double)parts * M * rows * 8 * 0.25e-6 : 0.;
-      const double us = (double)((tiles * parts + 255) / 256) * (each < steps ? each : steps) * mx_forms[f].us * (x8 ? 1. : 1.3) + planes;
-      if (us < best.us) best = {f, parts, each, false, 0, parts > 1 ? parts * (long long)M * (glu ? 2 : 1) * mx_pad(N) * 4 : 0, us};
+      const bool scales = odd && (each < steps ? each : steps) > 8;
+      const double us = (double)((tiles * parts + 255) / 256) * (each < steps ? each : steps) * mx_forms[f].us * (x8 ? 1. : 1.3) + planes +
+                        (scales ? 2.5 : 0.);
+      if (us < best.us) best = {f, parts, each, scales, 0, parts > 1 ? parts * (long long)M * (glu ? 2 : 1) * mx_pad(N) * 4 : 0, us};
     }
   }
-  best.scales = K % 512 != 0 || !aligned;
   best.scale_bytes = best.scales ? ((x8 ? (long long)M : 0) + rows) * mx_step(K) : 0;
   best.bytes += best.scale_bytes;
   return best;
@@ -787,7 +806,7 @@ static int mx_tiles(const char* what, hipStream_t stream, const MxGemm& g, void*
   TA_REQUIRE(plan.bytes == 0 || (scratch && scratch_bytes >= plan.bytes && (uintptr_t)scratch % 16 == 0),
              "%s: %lld bytes of scratch, %lld are needed", what, scratch ? scratch_bytes : 0LL, plan.bytes);
   TA_REQUIRE((rows + 256) * (g.K / 2) <= 0xffffffffLL || !GLU, "%s: gates and ups of %d x %d lie more than 4 GB apart", what, g.N, g.K);
-  MxTiles z = {g.xs, g.scales, g.K / MX_BLOCK, 0, 0, plan.parts, plan.part_steps, nullptr};
+  MxTiles z = {g.xs, g.scales, g.K % 512 == 0 && aligned ? g.K / MX_BLOCK : 0, 0, 0, plan.parts, plan.part_steps, nullptr};
   if (plan.scales) {
     z.step = mx_step(g.K);
     const long long xrows = X8 ? g.M : 0, grid = ((xrows + rows) * z.step / 4 + 255) / 256;
@@ -829,7 +848,7 @@ static bool mx_few(bool x8, bool glu, int M, int N, int K, bool aligned) {
   if (M > 64) return false;
   const MxPlan plan = mx_plan(x8, glu, M, N, K, aligned);
   const double weights = (double)N * (glu ? 2 : 1) * K * 1e-6;
-  return 2.3 + (M + 15) / 16 * weights * (x8 ? 0.20 : 0.24) < plan.us + 7. + (plan.scales ? 2.5 : 0.);
+  return 2.3 + (M + 15) / 16 * weights * (x8 ? 0.20 : 0.24) < plan.us + 7.;
 }
 
 // Bytes of scratch for M rows in 8 bits (x8) or bfloat16; aligned: all scales start on 16 bytes.
