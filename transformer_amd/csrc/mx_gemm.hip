@@ -34,14 +34,20 @@ struct MxGemm {
   int wide;                   // out is float32, else bfloat16
 };
 
-// COUNT neighbouring results of a row at out + at, `left` of them inside it; whole: all, and on 16 (8 where they are 4 bfloat16) bytes
+// Results go out in wide stores whatever the row's length leaves of their alignment (1,638 x 2,518 over k = 704, rows on 4 bytes, 12.4 us;
+// 16.3 a row at a time through LDS, 29 single)
+typedef mx_f32x4 mx_f32x4_any __attribute__((aligned(4)));
+typedef mx_u32x4 mx_u32x4_any __attribute__((aligned(2)));
+typedef mx_u32x2 mx_u32x2_any __attribute__((aligned(2)));
+
+// COUNT neighbouring results of a row at out + at, `left` of them inside it; whole: all
 template <int COUNT>
 __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const float* y, bool whole, int left) {
   if (g.wide) {
     float* o = (float*)g.out + at;
     if (whole) {
 #pragma unroll
-      for (int i = 0; i < COUNT; i += 4) *reinterpret_cast<mx_f32x4*>(o + i) = mx_f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+      for (int i = 0; i < COUNT; i += 4) *reinterpret_cast<mx_f32x4_any*>(o + i) = mx_f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
     } else {
 #pragma unroll
       for (int i = 0; i < COUNT; ++i)
@@ -54,12 +60,12 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const fl
 #pragma unroll
     for (int i = 0; i < COUNT; i += COUNT < 8 ? 4 : 8) {
       if (COUNT < 8) {
-        *reinterpret_cast<mx_u32x2*>(o + i) = mx_u32x2{f32x2_to_bf16x2_bits(y[i], y[i + 1]), f32x2_to_bf16x2_bits(y[i + 2], y[i + 3])};
+        *reinterpret_cast<mx_u32x2_any*>(o + i) = mx_u32x2{f32x2_to_bf16x2_bits(y[i], y[i + 1]), f32x2_to_bf16x2_bits(y[i + 2], y[i + 3])};
       } else {
         mx_u32x4 v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = f32x2_to_bf16x2_bits(y[(i + 2 * j) % COUNT], y[(i + 2 * j + 1) % COUNT]);
-        *reinterpret_cast<mx_u32x4*>(o + i) = v;
+        *reinterpret_cast<mx_u32x4_any*>(o + i) = v;
       }
     }
   } else {
@@ -652,22 +658,16 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
     return;
   }
   constexpr int CN = GLU ? 8 : 16;               // this lane's columns of the result
-  const int n_wave = n0 + wn * (4 * CN), n = n_wave + CN * q;
+  const int n = n0 + wn * (4 * CN) + CN * q;
   float add[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int c = i % CN;
     add[i] = g.bias && n + c < g.N ? g.bias[n + c + (i >= CN ? (long long)g.N : 0)] : 0.f;
   }
-  const bool pieces16 = g.ldo % (g.wide ? 4 : 8) == 0 && (uintptr_t)g.out % 16 == 0;
-  // rows that do not start on 16 bytes go through LDS (the wave's own, as far as it has just read it alone) and out a row at a time:
-  // single columns straight from the registers would be 64 places in memory a store (1,638 x 2,518 over k = 704 29 us)
-  constexpr int PAD = 4 * CN + 4;
-  float* mine = reinterpret_cast<float*>(mx_lds + part * (KG == 2 ? TM * 4096 : 16 * PAD * 4));
-  static_assert(16 * PAD * 4 <= (KG == 2 ? TM * 4096 : STAGE), "a wave's tile of results");
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
-    const int row0 = m0 + (wm * TM + m) * 16, row = row0 + r;
+    const int row = m0 + (wm * TM + m) * 16 + r;
     float y[CN];
 #pragma unroll
     for (int i = 0; i < CN; ++i) {
@@ -679,25 +679,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
         y[i] = v;
       }
     }
-    if (pieces16) {
-      if (row < g.M) mx_store<CN>(g, (long long)row * g.ldo + n, y, n + CN <= g.N, g.N - n);
-      continue;
-    }
-#pragma unroll
-    for (int i = 0; i < CN; i += 4)
-      *reinterpret_cast<mx_f32x4*>(mine + r * PAD + CN * q + i) = mx_f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; i += 16 / CN) {
-      const int at = i + lane / (4 * CN), c = lane % (4 * CN);
-      if (row0 + at < g.M && n_wave + c < g.N) {
-        const long long to = (long long)(row0 + at) * g.ldo + n_wave + c;
-        const float v = mine[at * PAD + c];
-        if (g.wide) reinterpret_cast<float*>(g.out)[to] = v;
-        else reinterpret_cast<bf16_t*>(g.out)[to] = from_f32<bf16_t>(v);
-      }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // read before the next tile overwrites it
+    if (row < g.M) mx_store<CN>(g, (long long)row * g.ldo + n, y, n + CN <= g.N, g.N - n);
   }
 }
 
@@ -721,8 +703,7 @@ __global__ __launch_bounds__(256) void mx_planes_kernel(MxGemm g, const float* _
   float y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = GLU ? v[0][i] / (1.0f + expf(-v[0][i])) * v[1][i] : v[0][i];
-  const bool whole = n + 4 <= g.N && g.ldo % 4 == 0 && (uintptr_t)g.out % 16 == 0;
-  mx_store<4>(g, (long long)row * g.ldo + n, y, whole, g.N - n);
+  mx_store<4>(g, (long long)row * g.ldo + n, y, n + 4 <= g.N, g.N - n);
 }
 
 // scales of rows of `blocks` bytes into rows of `step`, 127 behind them: k that is no multiple of 512 leaves rows off the 16
