@@ -238,6 +238,57 @@ def test_products_of_many_8_bit_rows(m, n, k):
     _close(got, U.values8(x.codes, x.scales), U.values4(w.codes, w.scales), ALIGNED)
 
 
+# more weights than groups of 16 rows pay for, in one part of k and in several; k off a step, off a load of scales, and with more
+# scales than LDS holds
+@pytest.mark.parametrize("n,k", [(8209, 4096), (4100, 14336), (7001, 5152), (33000, 1056), (33000, 8224)])
+@pytest.mark.parametrize("m", [18, 33, 64])
+def test_products_of_bfloat16_rows_with_many_weights(m, n, k):
+    w, x = _weights(n, k, 6), _randn(m, k, key=(6,)).bfloat16()
+    w64, bias = U.values4(w.codes, w.scales), _randn(n, key=(6,))
+    for dtype, b in ((torch.float32, bias), (torch.bfloat16, None)):
+        room = torch.full((m + 1, n + 7), 7.0, device=DEV, dtype=dtype)
+        got = kernels.gemm_mx4(x, w, room[:m, 3:n + 3], b)
+        assert bool((room[:, :3] == 7).all()) and bool((room[:, n + 3:] == 7).all()) and bool((room[m] == 7).all())
+        _close(got, x.double(), w64, 0.0, False, b)
+
+
+@pytest.mark.parametrize("n,k", [(4100, 4096), (2050, 14336), (3501, 5152), (16500, 1056), (16500, 8224)])
+@pytest.mark.parametrize("m", [19, 64])
+def test_gated_products_of_bfloat16_rows_with_many_weights(m, n, k):
+    w, x = _weights(2 * n, k, 7), _randn(m, k, key=(7,)).bfloat16()
+    bias = _randn(2 * n, key=(7,))
+    for dtype, b in ((torch.float32, bias), (torch.bfloat16, None)):
+        room = torch.full((m + 1, n + 7), 7.0, device=DEV, dtype=dtype)
+        got = kernels.gemm_mx4(x, w, room[:m, 3:n + 3], b, swiglu=True)
+        assert bool((room[:, :3] == 7).all()) and bool((room[:, n + 3:] == 7).all()) and bool((room[m] == 7).all())
+        _close(got, x.double(), U.values4(w.codes, w.scales), 0.0, True, b)
+
+
+def _off(t):
+    """The same values one byte behind a place on 16."""
+    room = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+    room[1:] = t.flatten()
+    return room[1:].view(t.shape)
+
+
+# scales off 16 bytes, by their rows' length or by where they start: every size of tile, with a part's scales in LDS at once or
+# laid out again
+@pytest.mark.parametrize("m,n,k", [(65, 128, 16416), (700, 1500, 4128), (1500, 2500, 2080), (1500, 4000, 2080), (2500, 4000, 2080),
+                                   (60, 33000, 8224), (90, 200, 2048), (1500, 2500, 2048), (1500, 4000, 2048), (2500, 4000, 2048)])
+def test_products_of_8_bit_rows_with_scales_off_16_bytes(m, n, k):
+    w, x = _weights(n, k, 5), _rows8(m, k, 5)
+    w, x = kernels.Mx4(w.codes, _off(w.scales)), kernels.Mx8(x.codes, _off(x.scales))
+    got = kernels.gemm_mx4(x, w, torch.empty(m, n, device=DEV, dtype=torch.bfloat16))
+    _close(got, U.values8(x.codes, x.scales), U.values4(w.codes, w.scales), ALIGNED)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 70, 2048), (40, 70, 2048), (40, 9000, 2048), (40, 33000, 8704)])
+def test_products_of_bfloat16_rows_with_scales_off_16_bytes(m, n, k):
+    w, x = _weights(n, k, 5), _randn(m, k, key=(5,)).bfloat16()
+    got = kernels.gemm_mx4(x, kernels.Mx4(w.codes, _off(w.scales)), torch.empty(m, n, device=DEV))
+    _close(got, x.double(), U.values4(w.codes, w.scales), 0.0)
+
+
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("m", [3, 40, 200])
 def test_whole_numbers_are_exact(m, eight):

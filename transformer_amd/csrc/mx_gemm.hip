@@ -306,9 +306,9 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
 }
 
 // ---------------------------------------------------------------- tiles of many rows
-// Tiles of BM rows by BN rows of the weights, k by steps of 128 (one scaled matrix instruction, or four on bfloat16). Both operands come into LDS without registers in
-// between, NS - 1 steps ahead, and so do the scales of every four steps (a row's are four bytes a step in a line of their own:
-// step by step they cost as many requests as the operands).
+// Tiles of BM rows by BN rows of the weights, k by steps of 128 (one scaled matrix instruction, or four on bfloat16). Both operands
+// come into LDS without registers in between, NS - 1 steps ahead, and so do the scales of every four steps (a row's are four bytes a
+// step in a line of their own: step by step they cost as many requests as the operands).
 //
 // Eight waves, two on every SIMD, in two groups half a phase apart: while one group reads its operands from LDS the other
 // multiplies, and a barrier ends the phase for both. KG 1: the groups are halves of the tile and take every step, in two phases;
@@ -324,8 +324,8 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
 // them in order and finishes. GLU: a tile holds 64 gates and their 64 ups, a lane's 16 columns are then 8 of either.
 __device__ __host__ __forceinline__ long long mx_pad(int n) { return (n + 3LL) / 4 * 4; }
 struct MxTiles {
-  const uint8_t *xs, *ws;     // scales in rows of `step` bytes, a multiple of 16, 127 behind the last block; or, with a step of 0, as
-  int step;                   // they are, and a part has 8 steps at most: a tile's scales come in through registers in front of them
+  const uint8_t *xs, *ws;     // scales in rows of `step` bytes, a multiple of 16, 127 behind the last block; step 0: as they are, rows
+  int step;                   // that do not start on 16 bytes, all of a part's brought through registers in front of its steps
   int m_tiles, n_tiles;
   int parts, part_steps;      // steps of a part, a multiple of 4
   float* planes;              // [parts][M][mx_pad(N), with GLU twice], or null
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
     if (X8) xs[m % HELD] = xsl[m * 256 + (r ^ ((wm * TM + m) & 3) * 4) * 16];
   };
   const auto read = [&](int step) {
-    const uint32_t sc = (step & 4) / 4 * GROUP + (step & 3) * 4;
+    const uint32_t sc = (z.step ? step >> 2 & 1 : step >> 2) * GROUP + (step & 3) * 4;
     const unsigned char *wl = mx_lds + (w_at + from), *wsl = mx_lds + (ws_at + sc);
     xl = mx_lds + (x_at + from);
     xsl = mx_lds + (xs_at + sc);
@@ -541,20 +541,30 @@ __global__ __launch_bounds__(512) void mx_tile_kernel(MxGemm g, MxTiles z) {
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) ask(i);
   if (!z.step) {
-    const int blocks = g.K / MX_BLOCK;
-    for (int at = threadIdx.x; at < 2 * (SX + BN); at += 512) {
-      const int half = at / (SX + BN), place = at % (SX + BN), row = place < SX ? place : place - SX, b = first * 4 + half * 16;
-      const uint8_t* from = place < SX ? z.xs + (size_t)(m0 + row < g.M ? m0 + row : g.M - 1) * blocks
-                                       : z.ws + ((size_t)n0 + weight_row(row)) * blocks;
-      mx_u32x4 v = {0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-      if (b + 16 <= blocks) {
-        __builtin_memcpy(&v, from + b, 16);
-      } else {
+    const int blocks = g.K / MX_BLOCK, count = (steps + 3) / 4 * (SX + BN);
+    for (int at = threadIdx.x; at < count; at += 4 * 512) {
+      mx_u32x4 v[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (b + i < blocks) v[i / 4] = (v[i / 4] & ~(255u << (8 * (i % 4)))) | (uint32_t)from[b + i] << (8 * (i % 4));
+      for (int j = 0; j < 4; ++j) {
+        const int place = (at + 512 * j) % (SX + BN), row = place < SX ? place : place - SX, b = (first + (at + 512 * j) / (SX + BN) * 4) * 4;
+        const uint8_t* from = place < SX ? z.xs + (size_t)(m0 + row < g.M ? m0 + row : g.M - 1) * blocks
+                                         : z.ws + ((size_t)n0 + weight_row(row)) * blocks;
+        v[j] = mx_u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+        if (at + 512 * j >= count) continue;
+        if (b + 16 <= blocks) {
+          __builtin_memcpy(&v[j], from + b, 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (b + i < blocks) v[j][i / 4] = (v[j][i / 4] & ~(255u << (8 * (i % 4)))) | (uint32_t)from[b + i] << (8 * (i % 4));
+        }
       }
-      *reinterpret_cast<mx_u32x4*>(mx_lds + AT_S + half * GROUP + (place ^ (place >> 4 & 3) * 4) * 16) = v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int place = (at + 512 * j) % (SX + BN);
+        if (at + 512 * j < count)
+          *reinterpret_cast<mx_u32x4*>(mx_lds + AT_S + (at + 512 * j) / (SX + BN) * GROUP + (place ^ (place >> 4 & 3) * 4) * 16) = v[j];
+      }
     }
   }
   end(0, NS - 2);
@@ -723,14 +733,17 @@ __global__ __launch_bounds__(256) void mx_scales_kernel(const uint8_t* __restric
 
 template <bool X8, bool GLU, int BM, int BN, int WM, int WN, int KG, int NS>
 static int mx_tile_launch(const char* what, hipStream_t stream, const MxGemm& g, MxTiles z) {
-  constexpr int steps = NS * (BM * (X8 ? 128 : 256) + BN * 64) + 2 * ((X8 ? BM : 0) + BN) * 16, sums = KG == 2 ? BM * BN * 4 : 0;
-  constexpr int bytes = steps > sums ? steps : sums;
-  static_assert(bytes <= MX_LDS, "a workgroup's LDS");
+  constexpr int steps = NS * (BM * (X8 ? 128 : 256) + BN * 64), scales = ((X8 ? BM : 0) + BN) * 16, sums = KG == 2 ? BM * BN * 4 : 0;
+  constexpr int most = steps + (MX_LDS - steps) / scales * scales;
+  static_assert(steps >= sums && steps + 2 * scales <= MX_LDS, "a workgroup's LDS");
+  const int all = (g.K + 127) / 128, each = z.part_steps < all ? z.part_steps : all;
+  const int bytes = steps + (z.step || each <= 8 ? 2 : (each + 3) / 4) * scales;
+  TA_REQUIRE(bytes <= most, "%s: scales of %d steps do not fit", what, each);
   const auto kernel = mx_tile_kernel<X8, GLU, BM, BN, WM, WN, KG, NS>;
   static bool asked = false;
-  if (!asked && bytes > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return ta_fail("%s: %d bytes of LDS refused (%s)", what, bytes, hipGetErrorString(e));
+  if (!asked) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != hipSuccess) return ta_fail("%s: %d bytes of LDS refused (%s)", what, most, hipGetErrorString(e));
     asked = true;
   }
   z.m_tiles = (g.M + BM - 1) / BM;
@@ -752,13 +765,16 @@ struct MxPlan {
 static const struct {
   int bm, bn;
   double us;
-} mx_forms[] = {{64, 128, 0.40}, {128, 128, 0.62}, {128, 256, 0.93}, {256, 256, 1.60}};
+  int held;                   // steps whose scales LDS holds at once
+} mx_forms[] = {{64, 128, 0.40, 64}, {128, 128, 0.62, 64}, {128, 256, 0.93, 40}, {256, 256, 1.60, 8}};
 static int mx_step(int K) { return (K + 511) / 512 * 16; }
 
 static MxPlan mx_plan(bool x8, bool glu, int M, int N, int K, bool aligned) {
   const long long rows = glu ? 2LL * N : N;
   const int steps = (K + 127) / 128;
-  const bool odd = K % 512 != 0 || !aligned;     // scales whose rows do not start on 16 bytes: laid out again, but where a part has few steps
+  // scales whose rows do not start on 16 bytes: all of a part's through registers at its start where LDS holds them, else laid out
+  // again by a kernel in front, a launch of 2.5 us (323 x 3,347 over k = 4,320: 18.3 and 20.6 us)
+  const bool odd = K % 512 != 0 || !aligned;
   MxPlan best = {};
   best.us = 1e30;
   for (int f = 0; f < (x8 ? 4 : 1); ++f) {
@@ -768,7 +784,7 @@ static MxPlan mx_plan(bool x8, bool glu, int M, int N, int K, bool aligned) {
       if (parts > 1 && (tiles * parts > 512 || (long long)(parts - 1) * each >= steps)) break;
       // planes are written and read once at some 4 TB/s, by a kernel of their own
       const double planes = parts > 1 ? 2.5 + (double)parts * M * rows * 8 * 0.25e-6 : 0.;
-      const bool scales = odd && (each < steps ? each : steps) > 8;
+      const bool scales = odd && (each < steps ? each : steps) > mx_forms[f].held;
       const double us = (double)((tiles * parts + 255) / 256) * (each < steps ? each : steps) * mx_forms[f].us * (x8 ? 1. : 1.3) + planes +
                         (scales ? 2.5 : 0.);
       if (us < best.us) best = {f, parts, each, scales, 0, parts > 1 ? parts * (long long)M * (glu ? 2 : 1) * mx_pad(N) * 4 : 0, us};
@@ -822,14 +838,15 @@ static int mx_gemm_check(const char* what, const MxGemm& g) {
 }
 
 // Whether the waves along k take it: up to 16 rows always; more in groups of 16, each of which reads the weights again, where that
-// is less than what the tiles cost (GPU time in us: 2.3 + 0.24, with 8 bits 0.20, for every million weights and group against the
-// tiles' steps, planes and scales and 7; 32 rows of 4,096 over k = 4,096 10 against 14, over 14,336 30 against 21).
+// is less than what the tiles cost (GPU time in us: 2.3 + 0.22, with 8 bits 0.17, for every million weights and group against the
+// tiles' steps, planes and scales and 4.5; of 13 shapes from 1,024 x 1,024 to 28,672 x 4,096 with 17, 32, 48 and 64 rows the faster
+// each time. 32 rows of 4,096 over k = 4,096 10.0 against 12.7, over 14,336 26.9 against 18.8).
 static bool mx_few(bool x8, bool glu, int M, int N, int K, bool aligned) {
   if (M <= 16) return true;
   if (M > 64) return false;
   const MxPlan plan = mx_plan(x8, glu, M, N, K, aligned);
   const double weights = (double)N * (glu ? 2 : 1) * K * 1e-6;
-  return 2.3 + (M + 15) / 16 * weights * (x8 ? 0.20 : 0.24) < plan.us + 7.;
+  return 2.3 + (M + 15) / 16 * weights * (x8 ? 0.17 : 0.22) < plan.us + 4.5;
 }
 
 // Bytes of scratch for M rows in 8 bits (x8) or bfloat16; aligned: all scales start on 16 bytes.
