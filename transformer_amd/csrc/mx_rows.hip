@@ -185,16 +185,49 @@ extern "C" int ta_swiglu_mx8(hipStream_t stream, int dtype, const void* gate_up,
 // v = x + delta (+ bias), stored to `stream` where there is one; y = v / sqrt(mean(v^2) + eps) * weight, to 8 bits. One
 // workgroup a row; HELD pieces of 8 values a thread stay in registers between the sum and the rows, 0: any number, read again
 // (by the thread that stored them).
+//
+// From v on everything is in 64 bits and rounded once, to e4m3: an error of 2^-24 common to a row moves one in some 10^6 of its
+// values over the middle between two codes, a sixteenth of itself away, and in 32 bits that is the largest error there is (2,048 rows of
+// 8,192: three times what v's own rounding leaves). 64 bits cost 1 of 39 us there.
+__device__ __forceinline__ double mx_sum64(double v) {
+  const auto take = [&](auto ctrl) {
+    const mx_u32x2 b = __builtin_bit_cast(mx_u32x2, v);
+    v += __builtin_bit_cast(double, mx_u32x2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)b[0], decltype(ctrl)::value, 0xf, 0xf, true),
+                                             (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b[1], decltype(ctrl)::value, 0xf, 0xf, true)});
+  };
+  take(std::integral_constant<int, 0xb1>());     // pairs, quads, halves of a row, rows
+  take(std::integral_constant<int, 0x4e>());
+  take(std::integral_constant<int, 0x141>());
+  take(std::integral_constant<int, 0x140>());
+  const mx_u32x2 b = __builtin_bit_cast(mx_u32x2, v);
+  double rows[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    rows[i] = __builtin_bit_cast(double, mx_u32x2{(uint32_t)__builtin_amdgcn_readlane((int)b[0], 16 * i),
+                                                  (uint32_t)__builtin_amdgcn_readlane((int)b[1], 16 * i)});
+  return (rows[0] + rows[1]) + (rows[2] + rows[3]);
+}
+
+// to 32 bits by truncation with the last bit set where anything is lost: a rounding to fewer bits then goes as from y itself
+__device__ __forceinline__ float mx_odd(double y) {
+  const float near = (float)y;
+  const double back = near;
+  uint32_t bits = __float_as_uint(near);
+  bits -= fabs(back) > fabs(y) && !isinf(near);
+  bits |= back != y && !isinf(near);
+  return __uint_as_float(bits);
+}
+
 template <typename TD, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x, const TD* __restrict__ delta,
                                                                   long long plane, int planes, const float* __restrict__ bias,
                                                                   const float* __restrict__ weight, float eps, float* to,
-                                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int d) {
+                                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int d, double share) {
   const size_t base = (size_t)blockIdx.x * d;
   const int pieces = d / 8;
-  __shared__ float part[THREADS / 64];
+  __shared__ double part[THREADS / 64];
   float held[HELD ? HELD : 1][8];
-  float sum = 0.f;
+  double sum = 0.;
   const auto form = [&](int p, float* v) {
     mx_load8(x + base + p * 8, v);
     for (int j = 0; j < planes; ++j) {
@@ -214,7 +247,7 @@ __global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x
       reinterpret_cast<float4*>(to + base + p * 8)[1] = make_float4(v[4], v[5], v[6], v[7]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += v[i] * v[i];
+    for (int i = 0; i < 8; ++i) sum += (double)v[i] * v[i];
   };
   if (HELD) {
 #pragma unroll
@@ -225,18 +258,20 @@ __global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x
   } else {
     for (int p = threadIdx.x; p < pieces; p += THREADS) form(p, held[0]);
   }
-  sum = wave_sum(sum);
+  sum = mx_sum64(sum);
   if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = sum;
   __syncthreads();
-  float all = 0.f;
+  double all = 0.;
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) all += part[w];
-  const float r = rsqrtf(all / (float)d + eps);
+  // the unit's root, good to some 26 bits, and a step of Newton's; 0 and infinity stay as they are
+  const double mean = all * share + (double)eps, near = __builtin_amdgcn_rsq(mean), better = near * (1.5 - 0.5 * mean * near * near);
+  const double r = isnan(better) ? near : better;
   const auto leave = [&](int p, const float* v) {
     float w[8], y[8];
     mx_load8(weight + p * 8, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = v[i] * r * w[i];
+    for (int i = 0; i < 8; ++i) y[i] = mx_odd(v[i] * r * w[i]);
     mx8_store(y, codes + base + p * 8, scales + base / 32 + p / 4);
   };
   if (HELD) {
@@ -259,7 +294,7 @@ template <typename TD>
 static void launch_norm(hipStream_t stream, const float* x, const TD* delta, int planes, const float* bias, const float* weight, float eps,
                         float* to, uint8_t* codes, uint8_t* scales, int n, int d) {
   const long long plane = (long long)n * d;
-#define MX_NORM(T, H) add_rmsnorm_mx8_kernel<TD, T, H><<<n, T, 0, stream>>>(x, delta, plane, planes, bias, weight, eps, to, codes, scales, d)
+#define MX_NORM(T, H) add_rmsnorm_mx8_kernel<TD, T, H><<<n, T, 0, stream>>>(x, delta, plane, planes, bias, weight, eps, to, codes, scales, d, 1. / d)
   if (d <= 2048) MX_NORM(256, 1);
   else if (d <= 4096) MX_NORM(512, 1);
   else if (d <= 8192) MX_NORM(1024, 1);
