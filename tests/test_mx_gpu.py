@@ -118,7 +118,13 @@ def test_norm_into_8_bits(m, d, form):
     assert torch.equal(x, before if form in ("plain", "stream") else v)      # one float32 addition after the other
     if stream is not None:
         assert torch.equal(stream, v)
-    y = v.double()
+    y = x.double() if form in ("plain", "stream") else before.double()         # (x holds the sum by now)
+    for t in ([] if delta is None else [delta] if delta.dim() == 2 else list(delta)):
+        y = y + t.double()
+    if bias is not None:
+        y = y + bias.double()
+    if d > 32768:                                   # the stream is read again
+        y = v.double()
     y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + 1e-5) * w.double()
     # 64 bits up to the one rounding: 30 of 2^-53 for the sum, the root and the products, and a root from 22 bits on (an error e
     # leaves 1.5 e^2)

@@ -857,15 +857,15 @@ extern "C" long long ta_gemm_mx4_scratch(int x8, int swiglu, int M, int N, int K
 
 // bfloat16 rows x [M][ldx] (rows on 16 bytes), at most ta_mx4_max_rows of them; out_dtype float32 or bfloat16; swiglu: the weights are N
 // gate rows and N up rows. scratch: ta_gemm_mx4_scratch bytes on 16.
-#define MX_FEW_ROWS 64
-extern "C" int ta_mx4_max_rows() { return MX_FEW_ROWS; }
+#define MX4_MAX_ROWS 64
+extern "C" int ta_mx4_max_rows() { return MX4_MAX_ROWS; }
 extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const void* x, long long ldx, const void* codes, const void* scales,
                            const float* bias, void* out, long long ldo, int M, int N, int K, void* scratch, long long scratch_bytes) {
   static const char what[] = "ta_gemm_mx4";
   TA_REQUIRE(out_dtype == TA_F32 || out_dtype == TA_BF16, "%s: unknown dtype %d", what, out_dtype);
   const MxGemm g = {x, nullptr, (const uint8_t*)codes, (const uint8_t*)scales, bias, out, ldx, ldo, M, N, K, out_dtype == TA_F32};
   if (mx_gemm_check(what, g)) return 1;
-  TA_REQUIRE(M <= MX_FEW_ROWS, "%s: %d bfloat16 rows, at most %d", what, M, MX_FEW_ROWS);
+  TA_REQUIRE(M <= MX4_MAX_ROWS, "%s: %d bfloat16 rows, at most %d", what, M, MX4_MAX_ROWS);
   TA_REQUIRE(ldx >= K && ldx % 8 == 0, "%s: rows %lld apart do not start on 16 bytes", what, ldx);
   TA_REQUIRE(ldx <= 1 << 24 && K <= 1 << 23, "%s: rows %lld apart, k %d: at most 16,777,216 and 8,388,608", what, ldx, K);   // a tile's rows within 32 bits
   TA_REQUIRE(!swiglu || N <= 0x3fffffff, "%s: %d gates", what, N);

@@ -186,9 +186,10 @@ extern "C" int ta_swiglu_mx8(hipStream_t stream, int dtype, const void* gate_up,
 // workgroup a row; HELD pieces of 8 values a thread stay in registers between the sum and the rows, 0: any number, read again
 // (by the thread that stored them).
 //
-// From v on everything is in 64 bits and rounded once, to e4m3: an error of 2^-24 common to a row moves one in some 10^6 of its
-// values over the middle between two codes, a sixteenth of itself away, and in 32 bits that is the largest error there is (2,048 rows of
-// 8,192: three times what v's own rounding leaves). 64 bits cost 1 of 39 us there.
+// What becomes the rows is added and normed in 64 bits beside the stream's 32 and rounded once, to e4m3: an error of 2^-24 moves one
+// in some 10^6 values over the middle between two codes, a sixteenth of itself away, and that would be the largest error there is.
+// It costs 3 of 42 us (2,048 rows of 8,192 with a bias: conversions, a quarter of the rate). Without registers for a row's pieces the
+// norm goes by the stream's values.
 __device__ __forceinline__ double mx_sum64(double v) {
   const auto take = [&](auto ctrl) {
     const mx_u32x2 b = __builtin_bit_cast(mx_u32x2, v);
@@ -226,28 +227,39 @@ __global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x
   const size_t base = (size_t)blockIdx.x * d;
   const int pieces = d / 8;
   __shared__ double part[THREADS / 64];
-  float held[HELD ? HELD : 1][8];
+  double held[HELD ? HELD : 1][8];
   double sum = 0.;
-  const auto form = [&](int p, float* v) {
+  const auto form = [&](int p, double* wide) {
+    float v[8];
     mx_load8(x + base + p * 8, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wide[i] = v[i];
+    const auto add = [&](const float* t) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] += t[i];
+        wide[i] += t[i];
+      }
+    };
     for (int j = 0; j < planes; ++j) {
       float t[8];
       mx_load8(delta + j * plane + base + p * 8, t);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += t[i];
+      add(t);
     }
     if (bias) {
       float t[8];
       mx_load8(bias + p * 8, t);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += t[i];
+      add(t);
     }
     if (to) {
       reinterpret_cast<float4*>(to + base + p * 8)[0] = make_float4(v[0], v[1], v[2], v[3]);
       reinterpret_cast<float4*>(to + base + p * 8)[1] = make_float4(v[4], v[5], v[6], v[7]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += (double)v[i] * v[i];
+    for (int i = 0; i < 8; ++i) {
+      if (!HELD) wide[i] = v[i];
+      sum += wide[i] * wide[i];
+    }
   };
   if (HELD) {
 #pragma unroll
@@ -267,7 +279,7 @@ __global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x
   // the unit's root, good to some 26 bits, and a step of Newton's; 0 and infinity stay as they are
   const double mean = all * share + (double)eps, near = __builtin_amdgcn_rsq(mean), better = near * (1.5 - 0.5 * mean * near * near);
   const double r = isnan(better) ? near : better;
-  const auto leave = [&](int p, const float* v) {
+  const auto leave = [&](int p, const double* v) {
     float w[8], y[8];
     mx_load8(weight + p * 8, w);
 #pragma unroll
@@ -285,7 +297,9 @@ __global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x
     for (int p = threadIdx.x; p < pieces; p += THREADS) {
       float v[8];
       mx_load8(from + base + p * 8, v);
-      leave(p, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) held[0][i] = v[i];
+      leave(p, held[0]);
     }
   }
 }

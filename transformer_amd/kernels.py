@@ -3036,8 +3036,8 @@ def swiglu_mx8(gate_up: torch.Tensor, out: Mx8, bias: Optional[torch.Tensor] = N
 def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8, delta: Optional[torch.Tensor] = None,
                     delta_bias: Optional[torch.Tensor] = None, stream: Optional[torch.Tensor] = None) -> Mx8:
     """``add_rmsnorm`` with the normed rows left in 8 bits: v = x + delta + delta_bias goes back to x (to ``stream`` where one
-    is given, which then gets v also when nothing is added), rmsnorm(v) * weight to out. delta float32 or bfloat16 [m, d], or
-    [planes, m, d] whose planes are added in order."""
+    is given, which then gets v also when nothing is added), rmsnorm(v) * weight to out, summed and normed in 64 bits (rows of
+    more than 32,768: from v as stored). delta float32 or bfloat16 [m, d], or [planes, m, d] whose planes are added in order."""
     m, d = out.shape
     at = torch._C._cuda_getDevice()
     code = planes = dp = 0
