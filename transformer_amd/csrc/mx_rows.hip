@@ -309,6 +309,8 @@ static void launch_norm(hipStream_t stream, const float* x, const TD* delta, int
                         float* to, uint8_t* codes, uint8_t* scales, int n, int d) {
   const long long plane = (long long)n * d;
 #define MX_NORM(T, H) add_rmsnorm_mx8_kernel<TD, T, H><<<n, T, 0, stream>>>(x, delta, plane, planes, bias, weight, eps, to, codes, scales, d, 1. / d)
+  // as many threads as a row has pieces: 8 x 8,192 3.9 us (with 512 threads of two pieces 4.4), 2,048 x 8,192 39.8 (40.6), 2,048 x 4,096
+  // 22.2 (with 256 threads of two 23.3)
   if (d <= 2048) MX_NORM(256, 1);
   else if (d <= 4096) MX_NORM(512, 1);
   else if (d <= 8192) MX_NORM(1024, 1);
