@@ -399,6 +399,59 @@ def test_chain_captured_replayed_and_on_another_stream():
             assert torch.equal(t, v), turn
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_two_graphs_whose_products_are_cut_in_parts_run_at_once(eight):
+    """Sums of a cut k go through scratch: two recorded products on two streams at once each keep their own."""
+    m, n, k = 40, 4096, 14336
+    assert kernels.gemm_mx4_scratch(eight, False, m, n, k) > 0
+    runs = []
+    for seed in (11, 12):
+        w, x = _weights(n, k, seed), _rows8(m, k, seed) if eight else _randn(m, k, key=(seed,)).bfloat16()
+        out = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)
+        want = kernels.gemm_mx4(x, w, out).clone()
+        _close(want, U.values8(x.codes, x.scales) if eight else x.double(), U.values4(w.codes, w.scales), ALIGNED if eight else 0.0)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                kernels.gemm_mx4(x, w, out)
+        runs.append((graph, torch.cuda.Stream(), out, want, w, x))
+    for _ in range(3):
+        for _, _, out, *_ in runs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream, *_ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, out, want, *_ in runs:
+            assert torch.equal(out, want)
+
+
+def test_more_elements_than_32_bits_count():
+    m, n, k = 70000, 32768, 64
+    w, x = _weights(n, k, 13), _rows8(m, k, 13)
+    y = kernels.gemm_mx4(x, w, torch.empty(m, n, device=DEV, dtype=torch.bfloat16))
+    for at in (0, 65535, 65536, m - 1):                       # 2^31 elements end in row 65,535
+        _close(y[at:at + 1], U.values8(x.codes[at:at + 1], x.scales[at:at + 1]), U.values4(w.codes, w.scales), ALIGNED)
+    rows = kernels.mx8_pack(y, kernels.Mx8.empty(m, n, DEV))
+    half = kernels.swiglu_mx8(y, kernels.Mx8.empty(m, n // 2, DEV))
+    for at in (65535, m - 1):
+        part = slice(at, at + 1)
+        v, b = U.pack8(y[part].double())
+        assert torch.equal(rows.scales[part], b) and torch.equal(rows.codes[part].float().double(), v)
+        gate, up = y[part].double().chunk(2, 1)
+        _check_rows(kernels.Mx8(half.codes[part], half.scales[part]), gate * torch.sigmoid(gate) * up, 6 * 2.0 ** -23)
+    del half
+    stream = torch.empty(m, n, device=DEV).normal_(generator=_gen(13))
+    last = stream[m - 1:].clone()
+    weight = 1 + 0.1 * _randn(n, key=(13,))
+    kernels.add_rmsnorm_mx8(stream, weight, 1e-5, rows, y)
+    assert torch.equal(stream[m - 1:], last + y[m - 1:].float())
+    v = last.double() + y[m - 1:].double()
+    v = v / torch.sqrt((v * v).mean(-1, keepdim=True) + 1e-5) * weight.double()
+    _check_rows(kernels.Mx8(rows.codes[m - 1:], rows.scales[m - 1:]), v, 2.0 ** -42)
+
+
 # ------------------------------------------------------------------ refusals
 def test_nothing_to_do():
     w = _weights(40, 64)
