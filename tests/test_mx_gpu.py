@@ -271,6 +271,21 @@ def test_gated_products_of_bfloat16_rows_with_many_weights(m, n, k):
         _close(got, x.double(), U.values4(w.codes, w.scales), 0.0, True, b)
 
 
+# as many columns as make a workgroup take 32: with a last one whose second 16 are there in part, or not at all
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("n,k", [(6157, 96), (8180, 544), (6160, 1056), (33000, 160), (4090, 2080), (28700, 4096)])
+@pytest.mark.parametrize("m", [5, 8, 9, 16, 17, 30, 64])
+def test_products_of_few_rows_with_many_columns(m, n, k, eight):
+    w, x = _weights(n, k, 14), _rows8(m, k, 14) if eight else _randn(m, k, key=(14,)).bfloat16()
+    bias = _randn(n, key=(14,))
+    x64, w64 = U.values8(x.codes, x.scales) if eight else x.double(), U.values4(w.codes, w.scales)
+    for dtype, b in ((torch.bfloat16, None), (torch.bfloat16 if eight else torch.float32, bias)):
+        room = torch.full((m + 1, n + 7), 7.0, device=DEV, dtype=dtype)
+        got = kernels.gemm_mx4(x, w, room[:m, 3:n + 3], b)
+        assert bool((room[:, :3] == 7).all()) and bool((room[:, n + 3:] == 7).all()) and bool((room[m] == 7).all())
+        _close(got, x64, w64, ALIGNED if eight else 0.0, False, b)
+
+
 def _off(t):
     """The same values one byte behind a place on 16."""
     room = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)

@@ -76,7 +76,7 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const fl
 }
 
 // ---------------------------------------------------------------- few rows
-// A workgroup owns 16 rows of the weights (with GLU 16 gates and their ups) and up to 16 rows of x; its waves deal k out among
+// A workgroup owns 16 rows of the weights (or 32, T 2; with GLU 16 gates and their ups) and up to 16 rows of x; its waves deal k out among
 // them in chunks of 128 S and their sums meet in LDS in wave order. A load of the weights brings whole lines, eight blocks of
 // eight rows; the matrix instruction wants four blocks of sixteen, so the halves of every sixteen lanes trade places between the
 // loads of rows 0 to 7 and 8 to 15 (a move across lanes for each register, no LDS). x goes
@@ -92,7 +92,7 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const fl
 // Measured (GPU time): 8-bit rows, 1 x 28,672 x 4,096 12.9 us (4.8 TB/s of a copy's 5.1), 8 rows 17.1, 16 rows 21.9, where x through LDS
 // costs as much as the weights; bfloat16 rows 1 x 4,096 x 4,096 4.7 (launch, one way to memory, the sums), 1 x 4,096 x 14,336 8.7, gated
 // 1 x 14,336 x 4,096 16.2 (3.9 TB/s: an instruction for every two codes).
-template <bool X8, bool GLU, int S, int R>
+template <bool X8, bool GLU, int S, int R, int T>
 __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
   if (gridDim.y > 1) {                          // this workgroup's R rows
     const long long at = (long long)blockIdx.y * R;
@@ -104,27 +104,33 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
   static_assert(R <= 16 && (S == 2 || S == 4), "rows of a tile, loads in pairs");
   constexpr int P = (X8 ? 8 : 16) * S;          // 16-byte pieces of a row of x in a chunk
   constexpr int FLIP = P < 16 ? P - 1 : 15;
-  constexpr int NT = GLU ? 2 : 1;               // tiles of the weights
+  constexpr int NT = GLU ? 2 : T;               // tiles of the weights: gates and ups, or neighbours
+  static_assert(!GLU || T == 1, "16 gates");
   constexpr int XI = R * P > 64 ? R * P / 64 : 1;               // loads of x
   constexpr int LOADS = XI + NT * (S + 1) + (X8 ? 1 : 0);       // of a chunk: at least so many
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   // (what is the same in a whole wave is told to be: addresses are then one base and 32 bits a lane)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, q = lane / 16,
             waves = blockDim.x / 64;
-  const int n0 = blockIdx.x * 16, blocks = g.K / MX_BLOCK, chunks = blocks / (4 * S);
+  const int n0 = blockIdx.x * (16 * T), blocks = g.K / MX_BLOCK, chunks = blocks / (4 * S);
   unsigned char* mine = mx_lds + wave * bytes;
   const uint8_t *codes[NT], *scales[NT];        // of the workgroup's first row, of its first ups
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    codes[t] = g.codes + ((size_t)n0 + (t ? (size_t)g.N : 0)) * (g.K / 2);
-    scales[t] = g.scales + ((size_t)n0 + (t ? (size_t)g.N : 0)) * blocks;
+    codes[t] = g.codes + ((size_t)n0 + (GLU && t ? (size_t)g.N : 0)) * (g.K / 2);
+    scales[t] = g.scales + ((size_t)n0 + (GLU && t ? (size_t)g.N : 0)) * blocks;
   }
-  const uint32_t col = n0 + r < g.N ? r : g.N - 1 - n0;         // this lane's row of the weights, from n0 on
-  uint32_t piece_at[2];                         // what it loads: a block of row r % 8, of row 8 + r % 8
+  uint32_t col[T];                              // this lane's rows of the weights, from n0 on
+  uint32_t piece_at[T][2];                      // what it loads: a block of row r % 8, of row 8 + r % 8
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int at = 8 * h + r % 8;
-    piece_at[h] = (uint32_t)(n0 + at < g.N ? at : g.N - 1 - n0) * (uint32_t)(g.K / 2) + (q + 4 * (r / 8)) * 16;
+  for (int t = 0; t < T; ++t) {
+    const int last = g.N - 1 - n0;
+    col[t] = 16 * t + r < last ? 16 * t + r : last;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = 16 * t + 8 * h + r % 8;
+      piece_at[t][h] = (uint32_t)(at < last ? at : last) * (uint32_t)(g.K / 2) + (q + 4 * (r / 8)) * 16;
+    }
   }
   const uint32_t row = r < g.M ? r : g.M - 1;   // and of x
   const uint32_t xstep = (uint32_t)g.ldx * (X8 ? 1 : 2);
@@ -147,11 +153,11 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
     if (X8) __builtin_memcpy(xs[set], g.xs + (size_t)c * 4 * S + row * (uint32_t)blocks, 4 * S);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      __builtin_memcpy(ws[set][t], scales[t] + (size_t)c * 4 * S + col * (uint32_t)blocks, 4 * S);
+      __builtin_memcpy(ws[set][t], scales[t] + (size_t)c * 4 * S + col[t % T] * (uint32_t)blocks, 4 * S);
 #pragma unroll
       for (int s = 0; s < S; ++s)
         w[set][t][s] = __builtin_nontemporal_load(
-            reinterpret_cast<const mx_u32x4*>(codes[t] + (size_t)(c * S + s / 2 * 2) * 64 + piece_at[s % 2]));
+            reinterpret_cast<const mx_u32x4*>(codes[t] + (size_t)(c * S + s / 2 * 2) * 64 + piece_at[t % T][s % 2]));
     }
   };
   // loads 2 i and 2 i + 1 to operands of steps 2 i and 2 i + 1: lanes 8 to 15 of the first take the second's of lanes 0 to 7,
@@ -247,8 +253,8 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
         w[0][t][s] = mx_u32x4{0, 0, 0, 0};
         ws[0][t][s] = 0x7f7f7f7fu;
         if (live) {
-          w[0][t][s] = *reinterpret_cast<const mx_u32x4*>(codes[t] + (size_t)b * 16 + col * (uint32_t)(g.K / 2));
-          ws[0][t][s] = (uint32_t)scales[t][b + col * (uint32_t)blocks] * 0x01010101u;
+          w[0][t][s] = *reinterpret_cast<const mx_u32x4*>(codes[t] + (size_t)b * 16 + col[t % T] * (uint32_t)(g.K / 2));
+          ws[0][t][s] = (uint32_t)scales[t][b + col[t % T] * (uint32_t)blocks] * 0x01010101u;
         }
       }
       if (X8) xs[0][s] = live ? (uint32_t)g.xs[b + row * (uint32_t)blocks] * 0x01010101u : 0x7f7f7f7fu;
@@ -263,17 +269,17 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[t * 256 + (q * 4 + i) * 16 + r] = acc[t][i];
   __syncthreads();
-  for (int at = threadIdx.x; at < 256; at += blockDim.x) {
-    const int m = at / 16, n = n0 + at % 16;
+  for (int at = threadIdx.x; at < 256 * T; at += blockDim.x) {
+    const int m = at % 256 / 16, n = n0 + at / 256 * 16 + at % 16;
     if (m >= g.M || n >= g.N) continue;
-    float v[NT];
+    float v[GLU ? 2 : 1];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < (GLU ? 2 : 1); ++t) {
       v[t] = 0.f;
       for (int wv = 0; wv < waves; ++wv) v[t] += reinterpret_cast<const float*>(mx_lds + wv * bytes)[t * 256 + at];
       if (g.bias) v[t] += g.bias[n + (long long)t * g.N];
     }
-    const float y = GLU ? v[0] / (1.0f + expf(-v[0])) * v[NT - 1] : v[0];
+    const float y = GLU ? v[0] / (1.0f + expf(-v[0])) * v[GLU ? 1 : 0] : v[0];
     const long long to = (long long)m * g.ldo + n;
     if (g.wide) reinterpret_cast<float*>(g.out)[to] = y;
     else reinterpret_cast<bf16_t*>(g.out)[to] = from_f32<bf16_t>(y);
@@ -281,11 +287,11 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
 }
 
 #define MX_LDS (160 * 1024)
-template <bool X8, bool GLU, int S, int R>
+template <bool X8, bool GLU, int S, int R, int T = 1>
 static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) {
-  constexpr int x = R * (X8 ? 8 : 16) * S * 16, sums = (GLU ? 2 : 1) * 1024;
-  const auto kernel = mx_few_kernel<X8, GLU, S, R>;
-  const int chunks = g.K / (128 * S), grid = (g.N + 15) / 16;
+  constexpr int x = R * (X8 ? 8 : 16) * S * 16, sums = (GLU ? 2 : T) * 1024;
+  const auto kernel = mx_few_kernel<X8, GLU, S, R, T>;
+  const int chunks = g.K / (128 * S), grid = (g.N + 16 * T - 1) / (16 * T);
   // as many waves as give every CU 16, then the fewest that need as many turns; one buffer of x does for one turn
   int waves = (16 * 256 + grid - 1) / grid;
   waves = waves < 4 ? 4 : waves > 16 ? 16 : waves;
@@ -843,16 +849,34 @@ static int mx_gemm_check(const char* what, const MxGemm& g) {
   return 0;
 }
 
-// Whether the waves along k take it: up to 16 rows always; more in groups of 16, each of which reads the weights again, where that
-// is less than what the tiles cost (GPU time in us: 2.3 + 0.22, with 8 bits 0.17, for every million weights and group against the
-// tiles' steps, planes and scales and 4.5; of 13 shapes from 1,024 x 1,024 to 28,672 x 4,096 with 17, 32, 48 and 64 rows the faster
-// each time. 32 rows of 4,096 over k = 4,096 10.0 against 12.7, over 14,336 26.9 against 18.8).
+// What the waves along k take (GPU time in us, measured from 1,024 x 1,024 to 28,672 x 4,096 with 5 to 64 rows): 2.3 and, for every round of
+// 256 workgroups and 1,000 k, 0.55 with up to 8 rows of x, 0.68 with up to 16 in 8 bits and 0.88 in bfloat16; with 32 rows of the weights
+// (or 16 gates and their ups) a workgroup 0.95, 1.1 and 1.3.
+static double mx_few_us(bool x8, bool glu, bool pairs, int M, int N, int K) {
+  const int rows = pairs ? 32 : 16;
+  const double each = glu || pairs ? (M <= 8 ? 0.95 : x8 ? 1.1 : 1.3) : M <= 8 ? 0.55 : x8 ? 0.68 : 0.88;
+  return 2.3 + (double)((((long long)N + rows - 1) / rows * ((M + 15) / 16) + 255) / 256) * each * K * 1e-3;
+}
+
+// Whether a workgroup takes 32 rows of the weights and not 16: x then goes through LDS half as often, and there are half as many
+// workgroups (64 bfloat16 rows of 4,096 over k = 4,096 12.3 us and 16.0, 16 of 6,144 7.5 and 9.8, 16 of 28,672 22.2 and 26.4; 16 of 4,096,
+// where 256 workgroups are one round, 7.4 and 5.7)
+static bool mx_few_pairs(bool x8, int M, int N, int K) {
+  return M > 4 && mx_few_us(x8, false, true, M, N, K) < 0.97 * mx_few_us(x8, false, false, M, N, K);
+}
+
+// Whether the waves along k take it: up to 4 rows always; more, in groups of 16 each of which reads the weights again, where that
+// is less than what the tiles cost, their steps, planes and scales and 4.5 (32 bfloat16 rows of 4,096 over k = 4,096 7.4 us against 12.7, of
+// 14,336 over 4,096 25 against 17). Up to 16 rows it stays with them where tiles want scratch, which a caller then need not ask
+// about (8-bit rows, 16 of 28,672 19.9 us against 15.3).
 static bool mx_few(bool x8, bool glu, int M, int N, int K, bool aligned) {
-  if (M <= 16) return true;
+  if (M <= 4) return true;
   if (M > 64) return false;
+  double us = mx_few_us(x8, glu, false, M, N, K);
+  if (!glu && mx_few_pairs(x8, M, N, K)) us = mx_few_us(x8, false, true, M, N, K);
+  if (M <= 16 && us < 12.) return true;          // (tiles without scratch are hardly less)
   const MxPlan plan = mx_plan(x8, glu, M, N, K, aligned);
-  const double weights = (double)N * (glu ? 2 : 1) * K * 1e-6;
-  return 2.3 + (M + 15) / 16 * weights * (x8 ? 0.17 : 0.22) < plan.us + 4.5;
+  return us < plan.us + 4.5 || (M <= 16 && plan.bytes);
 }
 
 // Bytes of scratch for M rows in 8 bits (x8) or bfloat16; aligned: all scales start on 16 bytes.
@@ -888,6 +912,7 @@ extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const 
   }
   if (M <= 1) return mx_few_launch<false, false, 4, 1>(what, stream, g);
   if (M <= 4) return mx_few_launch<false, false, 4, 4>(what, stream, g);
+  if (mx_few_pairs(false, M, N, K)) return M <= 8 ? mx_few_launch<false, false, 2, 8, 2>(what, stream, g) : mx_few_launch<false, false, 2, 16, 2>(what, stream, g);
   if (M <= 8) return mx_few_launch<false, false, 4, 8>(what, stream, g);
   return mx_few_launch<false, false, 2, 16>(what, stream, g);
 }
@@ -904,6 +929,7 @@ extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs
   // (1 x 28,672 x 4,096 in chunks of 512 11.8 us, of 256 14.9; 16 rows 21.7 and 20.9)
   if (M <= 1) return mx_few_launch<true, false, 4, 1>(what, stream, g);
   if (M <= 4) return mx_few_launch<true, false, 4, 4>(what, stream, g);
+  if (mx_few_pairs(true, M, N, K)) return M <= 8 ? mx_few_launch<true, false, 2, 8, 2>(what, stream, g) : mx_few_launch<true, false, 2, 16, 2>(what, stream, g);
   if (M <= 8) return mx_few_launch<true, false, 2, 8>(what, stream, g);
   return mx_few_launch<true, false, 2, 16>(what, stream, g);
 }
