@@ -89,9 +89,9 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const fl
 // Waves: every CU wants some 16 of them with two chunks each on their way, which 64 KB of weights in flight keep the memory
 // busy with; fewer than four a workgroup leave too many of the sums' exchanges.
 //
-// Measured (GPU time): 8-bit rows, 1 x 28,672 x 4,096 12.9 us (4.8 TB/s of a copy's 5.1), 8 rows 17.1, 16 rows 21.9, where x through LDS
-// costs as much as the weights; bfloat16 rows 1 x 4,096 x 4,096 4.7 (launch, one way to memory, the sums), 1 x 4,096 x 14,336 8.7, gated
-// 1 x 14,336 x 4,096 16.2 (3.9 TB/s: an instruction for every two codes).
+// Measured (GPU time): 8-bit rows, 1 x 28,672 x 4,096 12.9 us (4.8 TB/s of a copy's 5.1), 8 x 14,336 x 4,096 9.7, 16 rows 10.8, where x
+// through LDS costs as much as the weights; bfloat16 rows 1 x 4,096 x 4,096 4.7 (launch, one way to memory, the sums), 1 x 4,096 x 14,336
+// 8.7, 8 x 4,096 x 14,336 10.5, gated 1 x 14,336 x 4,096 16.2 (3.9 TB/s: an instruction for every two codes).
 template <bool X8, bool GLU, int S, int R, int T>
 __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
   if (gridDim.y > 1) {                          // this workgroup's R rows
@@ -865,18 +865,16 @@ static bool mx_few_pairs(bool x8, int M, int N, int K) {
   return M > 4 && mx_few_us(x8, false, true, M, N, K) < 0.97 * mx_few_us(x8, false, false, M, N, K);
 }
 
-// Whether the waves along k take it: up to 4 rows always; more, in groups of 16 each of which reads the weights again, where that
-// is less than what the tiles cost, their steps, planes and scales and 4.5 (32 bfloat16 rows of 4,096 over k = 4,096 7.4 us against 12.7, of
-// 14,336 over 4,096 25 against 17). Up to 16 rows it stays with them where tiles want scratch, which a caller then need not ask
-// about (8-bit rows, 16 of 28,672 19.9 us against 15.3).
+// Whether the waves along k take it: up to 16 rows always (a step of the 8B shape at batch 8 with 8-bit rows 3,560 tokens a second, with tiles
+// for 28,672 columns 3,380: out of memory they come slower); more, in groups of 16 each of which reads the weights again, where that is
+// less than what the tiles cost, their steps, planes and scales and 4.5 (32 bfloat16 rows of 4,096 over k = 4,096 7.4 us against 12.7, of
+// 14,336 over 4,096 25 against 17).
 static bool mx_few(bool x8, bool glu, int M, int N, int K, bool aligned) {
-  if (M <= 4) return true;
+  if (M <= 16) return true;
   if (M > 64) return false;
   double us = mx_few_us(x8, glu, false, M, N, K);
   if (!glu && mx_few_pairs(x8, M, N, K)) us = mx_few_us(x8, false, true, M, N, K);
-  if (M <= 16 && us < 12.) return true;          // (tiles without scratch are hardly less)
-  const MxPlan plan = mx_plan(x8, glu, M, N, K, aligned);
-  return us < plan.us + 4.5 || (M <= 16 && plan.bytes);
+  return us < mx_plan(x8, glu, M, N, K, aligned).us + 4.5;
 }
 
 // Bytes of scratch for M rows in 8 bits (x8) or bfloat16; aligned: all scales start on 16 bytes.
@@ -897,7 +895,8 @@ extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const 
   if (mx_gemm_check(what, g)) return 1;
   TA_REQUIRE(M <= MX4_MAX_ROWS, "%s: %d bfloat16 rows, at most %d", what, M, MX4_MAX_ROWS);
   TA_REQUIRE(ldx >= K && ldx % 8 == 0, "%s: rows %lld apart do not start on 16 bytes", what, ldx);
-  TA_REQUIRE(ldx <= 1 << 24 && K <= 1 << 23, "%s: rows %lld apart, k %d: at most 16,777,216 and 8,388,608", what, ldx, K);   // a tile's rows within 32 bits
+  // (a tile's rows within 32 bits)
+  TA_REQUIRE(ldx <= 1 << 24 && K <= 1 << 23, "%s: rows %lld apart, k %d: at most 16,777,216 and 8,388,608", what, ldx, K);
   TA_REQUIRE(!swiglu || N <= 0x3fffffff, "%s: %d gates", what, N);
   if (M == 0) return 0;
   if (!mx_few(false, swiglu, M, N, K, (uintptr_t)scales % 16 == 0))
@@ -912,7 +911,8 @@ extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const 
   }
   if (M <= 1) return mx_few_launch<false, false, 4, 1>(what, stream, g);
   if (M <= 4) return mx_few_launch<false, false, 4, 4>(what, stream, g);
-  if (mx_few_pairs(false, M, N, K)) return M <= 8 ? mx_few_launch<false, false, 2, 8, 2>(what, stream, g) : mx_few_launch<false, false, 2, 16, 2>(what, stream, g);
+  if (mx_few_pairs(false, M, N, K))
+    return M <= 8 ? mx_few_launch<false, false, 2, 8, 2>(what, stream, g) : mx_few_launch<false, false, 2, 16, 2>(what, stream, g);
   if (M <= 8) return mx_few_launch<false, false, 4, 8>(what, stream, g);
   return mx_few_launch<false, false, 2, 16>(what, stream, g);
 }
@@ -925,11 +925,13 @@ extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs
   if (mx_gemm_check(what, g)) return 1;
   TA_REQUIRE(K <= 1 << 23, "%s: k %d: at most 8,388,608", what, K);         // 256 rows within 31 bits
   if (M == 0) return 0;
-  if (!mx_few(true, false, M, N, K, ((uintptr_t)xs | (uintptr_t)scales) % 16 == 0)) return mx_tiles<true, false>(what, stream, g, scratch, scratch_bytes);
+  if (!mx_few(true, false, M, N, K, ((uintptr_t)xs | (uintptr_t)scales) % 16 == 0))
+    return mx_tiles<true, false>(what, stream, g, scratch, scratch_bytes);
   // (1 x 28,672 x 4,096 in chunks of 512 11.8 us, of 256 14.9; 16 rows 21.7 and 20.9)
   if (M <= 1) return mx_few_launch<true, false, 4, 1>(what, stream, g);
   if (M <= 4) return mx_few_launch<true, false, 4, 4>(what, stream, g);
-  if (mx_few_pairs(true, M, N, K)) return M <= 8 ? mx_few_launch<true, false, 2, 8, 2>(what, stream, g) : mx_few_launch<true, false, 2, 16, 2>(what, stream, g);
+  if (mx_few_pairs(true, M, N, K))
+    return M <= 8 ? mx_few_launch<true, false, 2, 8, 2>(what, stream, g) : mx_few_launch<true, false, 2, 16, 2>(what, stream, g);
   if (M <= 8) return mx_few_launch<true, false, 2, 8>(what, stream, g);
   return mx_few_launch<true, false, 2, 16>(what, stream, g);
 }
