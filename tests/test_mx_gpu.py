@@ -508,3 +508,14 @@ def test_what_is_refused():
                  lambda: kernels.Mx4.empty(4, 48, DEV), lambda: kernels.Mx8.empty(4, 48, DEV)):
         with pytest.raises(kernels.KernelError):
             call()
+
+
+def test_more_rows_than_a_launch_counts_are_refused():
+    m = 2 ** 32 + 5                                      # 5, in 32 bits
+    if torch.cuda.mem_get_info()[0] < 200e9:
+        pytest.skip("wants 150 GB")
+    rows = kernels.Mx8.empty(m, 32, DEV)
+    with pytest.raises(kernels.KernelError, match="2\\^31"):
+        kernels.gemm_mx4(rows, _weights(1, 32), torch.empty(m, 1, device=DEV, dtype=torch.bfloat16))
+    del rows
+    torch.cuda.empty_cache()

@@ -3130,6 +3130,8 @@ def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, 
         _rows2d(x, "a"); _rows2d(out, "out")
     if m == 0 or cols == 0:
         return out
+    if (m | n) >> 31:
+        raise KernelError(f"gemm_mx4: {m} rows against {n}: a call takes fewer than 2^31 of either")
     xs, ws = a.scales.data_ptr() if eight else 0, w.scales.data_ptr()
     scratch = need = 0
     if m > MX_FEW_ROWS:
