@@ -86,3 +86,37 @@ def test_a_launch_without_a_device_fails():
     for rc, name in ((_gemm(lib), b"ta_gemm_mx4"), (_gemm(lib, glu=1, M=40, **room), b"ta_gemm_mx4"), (_gemm8(lib), b"ta_gemm_mx4_mx8"),
                      (_gemm(lib, M=64, N=4096, K=14336, **room), b"ta_gemm_mx4"), (_gemm8(lib, M=600, N=1024, K=2048, **room), b"ta_gemm_mx4_mx8")):
         assert rc != 0 and lib.ta_last_error().startswith(name), lib.ta_last_error()
+
+
+def _packed(kind, n, k):
+    """An ``Mx4`` or ``Mx8`` without memory."""
+    t, (dtype, width) = object.__new__(kind), {kernels.Mx4: (torch.uint8, k // 2), kernels.Mx8: (torch.float8_e4m3fn, k)}[kind]
+    t.codes, t.scales = torch.empty(n, width, dtype=dtype, device="meta"), torch.empty(n, k // 32, dtype=torch.uint8, device="meta")
+    t.shape = (n, k)
+    return t
+
+
+def _bare(*shape, dtype=torch.float32):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("k", [2 ** 31, 2 ** 32, 2 ** 32 + 32, 2 ** 33 + 4096])
+def test_a_k_beyond_a_launchs_integers_is_refused(k, monkeypatch):
+    """The wrappers on tensors without memory, up to the launch, where 32 bits of such a k would pass as 0, 32 or 4,096."""
+    def launch(name):
+        raise AssertionError(f"{name} would be launched")
+    for name, stand_in in (("_dev", lambda t, *a, **kw: t), ("_here", lambda *a: None), ("_stream", lambda: None), ("_mx", launch)):
+        monkeypatch.setattr(kernels, name, stand_in)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)          # where such a tensor says that it is
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda at: 0, raising=False)
+    rows, w, bf = _packed(kernels.Mx8, 1, k), _packed(kernels.Mx4, 1, k), torch.bfloat16
+    for call in (lambda: kernels.mx4_pack(_bare(1, k, dtype=bf), w), lambda: kernels.mx4_unpack(w, _bare(1, k, dtype=bf)),
+                 lambda: kernels.mx8_pack(_bare(1, k), rows), lambda: kernels.swiglu_mx8(_bare(1, 2 * k, dtype=bf), rows),
+                 lambda: kernels.add_rmsnorm_mx8(_bare(1, k), _bare(k), 1e-5, rows),
+                 lambda: kernels.add_rmsnorm_mx8(_bare(k, 32), _bare(32), 1e-5, _packed(kernels.Mx8, k, 32)),
+                 lambda: kernels.add_rmsnorm_mx8(_bare(1, 32), _bare(32), 1e-5, _packed(kernels.Mx8, 1, 32), _bare(k + 1, 1, 32, dtype=bf)),
+                 lambda: kernels.gemm_mx4(rows, w, _bare(1, 1, dtype=bf)), lambda: kernels.gemm_mx4(_bare(1, k, dtype=bf), w, _bare(1, 1)),
+                 lambda: kernels.gemm_mx4_scratch(True, False, 64, 4096, k), lambda: kernels.gemm_mx4_scratch(True, False, k, 64, 4096),
+                 lambda: kernels.gemm_mx4_scratch(True, False, 64, k, 4096)):
+        with pytest.raises(kernels.KernelError, match="fewer than 2\\^31"):
+            call()

@@ -2907,6 +2907,10 @@ def _here(what: str, *tensors):
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{at}")
 
 
+def _too_large(what: str, **sizes):
+    raise KernelError(f"{what}: {', '.join(f'{n} {v}' for n, v in sizes.items())}: a launch counts each in 32 bits, fewer than 2^31")
+
+
 def _vector(t: Optional[torch.Tensor], n: int, at: int) -> bool:
     """Whether t is None or n float32 values in a row on the current device ``at``."""
     return t is None or (t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == at)
@@ -2987,6 +2991,8 @@ def mx4_pack(w: torch.Tensor, out: Mx4) -> Mx4:
     if tuple(w.shape) != out.shape:
         raise KernelError(f"mx4_pack: w {tuple(w.shape)} out {out.shape}")
     _here("mx4_pack", w, out.codes)
+    if w.shape[1] >> 31:
+        _too_large("mx4_pack", k=w.shape[1])
     _check(_mx("ta_mx4_pack")(_stream(), _code(w.dtype), w.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), n, w.shape[1]))
     return out
 
@@ -2998,6 +3004,8 @@ def mx4_unpack(w: Mx4, out: torch.Tensor) -> torch.Tensor:
     if tuple(out.shape) != w.shape:
         raise KernelError(f"mx4_unpack: w {w.shape} out {tuple(out.shape)}")
     _here("mx4_unpack", out, w.codes)
+    if w.shape[1] >> 31:
+        _too_large("mx4_unpack", k=w.shape[1])
     _check(_mx("ta_mx4_unpack")(_stream(), _code(out.dtype), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ld, n, w.shape[1]))
     return out
 
@@ -3010,6 +3018,8 @@ def mx8_pack(x: torch.Tensor, out: Mx8) -> Mx8:
     if tuple(x.shape) != out.shape:
         raise KernelError(f"mx8_pack: x {tuple(x.shape)} out {out.shape}")
     _here("mx8_pack", x, out.codes)
+    if x.shape[1] >> 31:
+        _too_large("mx8_pack", k=x.shape[1])
     _check(_mx("ta_mx8_pack")(_stream(), _code(x.dtype), x.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), m, x.shape[1]))
     return out
 
@@ -3026,6 +3036,8 @@ def swiglu_mx8(gate_up: torch.Tensor, out: Mx8, bias: Optional[torch.Tensor] = N
     ld, inner = gate_up.stride()
     if inner != 1:
         _rows2d(gate_up, "gate_up")
+    if d >> 31:
+        _too_large("swiglu_mx8", d=d)
     rc = _mx("ta_swiglu_mx8")(torch._C._cuda_getCurrentRawStream(at), _code(gate_up.dtype), gate_up.data_ptr(), ld,
                               None if bias is None else bias.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d)
     if rc:
@@ -3065,6 +3077,8 @@ def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8,
                           f"stream {None if stream is None else tuple(stream.shape)}")
     if m == 0:
         return out
+    if (m | d | planes) >> 31:
+        _too_large("add_rmsnorm_mx8", rows=m, d=d, planes=planes)
     rc = _mx("ta_add_rmsnorm_mx8")(torch._C._cuda_getCurrentRawStream(at), code, x.data_ptr(), dp or None, planes,
                                    None if delta_bias is None else delta_bias.data_ptr(), weight.data_ptr(), eps,
                                    None if stream is None else stream.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d)
@@ -3082,6 +3096,8 @@ def gemm_mx4_scratch(eight: bool, swiglu: bool, rows: int, n: int, k: int, align
     key = (eight, swiglu, rows, n, k, aligned)
     need = _mx_scratch_sizes.get(key)
     if need is None:
+        if (rows | n | k) >> 31:
+            _too_large("gemm_mx4_scratch", rows=rows, n=n, k=k)
         f = library().ta_gemm_mx4_scratch
         f.restype = c_longlong
         if len(_mx_scratch_sizes) > 4096:
@@ -3130,8 +3146,8 @@ def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, 
         _rows2d(x, "a"); _rows2d(out, "out")
     if m == 0 or cols == 0:
         return out
-    if (m | n) >> 31:
-        raise KernelError(f"gemm_mx4: {m} rows against {n}: a call takes fewer than 2^31 of either")
+    if (m | n | k) >> 31:
+        _too_large("gemm_mx4", rows=m, n=n, k=k)
     xs, ws = a.scales.data_ptr() if eight else 0, w.scales.data_ptr()
     scratch = need = 0
     if m > MX_FEW_ROWS:
