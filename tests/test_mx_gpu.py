@@ -166,6 +166,25 @@ def test_gated_activation_far_out():
     assert got[0] == 0 and got[2] == 0 and abs(got[3] / 1e30 - 1) <= 2.0 ** -4 and bool((got[4:] == 0).all())
 
 
+@pytest.mark.parametrize("far", [81.0, 200.0, -200.0, 1e30, float("inf"), float("nan")])
+def test_a_gate_far_out_changes_no_other_block(far):
+    """Rows of 96 values share waves: with one gate out of range in a row the other rows, and the other blocks of its own, keep their bits. The
+    values lie within a unit or two of 1.0625, the middle between two codes, so that a last bit of silu moves them."""
+    m, d = 1367, 96
+    g = 2 * _randn(m, d, key=(21,))
+    gu = torch.cat((g, (1.0625 / (g.double() * torch.sigmoid(g.double()))).float()), 1)
+    gu[:, 0:d:32], gu[:, d::32] = 3.0, 100.0        # a block's largest: 286, so the scale is 1
+    want = kernels.swiglu_mx8(gu, kernels.Mx8.empty(m, d, DEV))
+    assert bool((want.scales == 127).all())
+    odd = gu.clone()
+    odd[2::5, 40] = far                             # a wave of 512 values holds five rows and a third
+    got = kernels.swiglu_mx8(odd, kernels.Mx8.empty(m, d, DEV))
+    same = torch.ones(m, d // 32, dtype=torch.bool, device=DEV)
+    same[2::5, 1] = False
+    assert torch.equal(got.scales[same], want.scales[same])
+    assert torch.equal(_bits(got.codes).view(m, -1, 32)[same], _bits(want.codes).view(m, -1, 32)[same])
+
+
 # ------------------------------------------------------------------ products
 def _close(got, x, w, extra, glu=False, bias=None):
     """Within the result's rounding of the product in 64 bits, and float32 sums of k products: an addition is off by 2^-23 of the sum

@@ -156,15 +156,19 @@ __global__ __launch_bounds__(256) void swiglu_mx8_kernel(const T* __restrict__ g
       u[i] += bu[i];
     }
   }
-  // (NaN and infinities have bits above those of 80)
-  if (__any(mx_top8(g) > 0x42a00000u)) {
+  // a gate beyond 80 (NaN and infinities have bits above it too) goes by the library's functions, itself alone: a value's bits are its own
+  // gate's and up's, whatever else its row or its wave holds
+  float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
-  } else {
+  for (int i = 0; i < 8; ++i) y[i] = mx_silu(g[i]);
+  if (mx_top8(g) > 0x42a00000u) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = mx_silu(g[i]) * u[i];
+    for (int i = 0; i < 8; ++i)
+      if ((__float_as_uint(g[i]) & 0x7fffffffu) > 0x42a00000u) y[i] = g[i] / (1.0f + expf(-g[i]));
   }
-  mx8_store(g, codes + row * d + p * 8, scales + row * (d / 32) + p / 4);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] *= u[i];
+  mx8_store(y, codes + row * d + p * 8, scales + row * (d / 32) + p / 4);
 }
 
 // gate_up [n][ld] float32 or bfloat16: d gates, then d ups; bias [2 d] or null.
