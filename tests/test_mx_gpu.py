@@ -131,6 +131,22 @@ def test_norm_into_8_bits(m, d, form):
     _check_rows(out, y, 2.0 ** -42)
 
 
+def test_norm_of_more_rows_than_a_launch_has_threads_for():
+    """2^24 rows have 256 threads each, 2^32 in all: the first and the last rows, and those on both sides of a border of 2^21 rows."""
+    m, d = 2 ** 24 + 3, 32
+    x = torch.empty(m, d, device=DEV).normal_(generator=_gen(22))
+    delta = torch.empty(2, m, d, device=DEV, dtype=torch.bfloat16).normal_(generator=_gen(23))
+    w = 1 + 0.1 * _randn(d, key=(2,))
+    out, stream = kernels.Mx8.empty(m, d, DEV), torch.empty_like(x)
+    kernels.add_rmsnorm_mx8(x, w, 1e-5, out, delta, stream=stream)
+    assert torch.equal(stream, x + delta[0].float() + delta[1].float())
+    for at in (0, 2 ** 21 - 2, 7 * 2 ** 21 - 1, 2 ** 24 - 3):
+        part = slice(at, at + 6)
+        y = x[part].double() + delta[0, part].double() + delta[1, part].double()
+        y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + 1e-5) * w.double()
+        _check_rows(kernels.Mx8(out.codes[part], out.scales[part]), y, 2.0 ** -42)
+
+
 def test_norm_of_rows_that_hold_what_is_not_finite():
     x = _randn(4, 2080)
     x[1, 40], x[2, 70] = float("nan"), float("inf")

@@ -310,8 +310,7 @@ __global__ __launch_bounds__(THREADS) void add_rmsnorm_mx8_kernel(const float* x
 
 template <typename TD>
 static void launch_norm(hipStream_t stream, const float* x, const TD* delta, int planes, const float* bias, const float* weight, float eps,
-                        float* to, uint8_t* codes, uint8_t* scales, int n, int d) {
-  const long long plane = (long long)n * d;
+                        float* to, uint8_t* codes, uint8_t* scales, int n, int d, long long plane) {
 #define MX_NORM(T, H) add_rmsnorm_mx8_kernel<TD, T, H><<<n, T, 0, stream>>>(x, delta, plane, planes, bias, weight, eps, to, codes, scales, d, 1. / d)
   // as many threads as a row has pieces: 8 x 8,192 3.9 us (with 512 threads of two pieces 4.4), 2,048 x 8,192 39.8 (40.6), 2,048 x 4,096
   // 22.2 (with 256 threads of two 23.3)
@@ -334,10 +333,18 @@ extern "C" int ta_add_rmsnorm_mx8(hipStream_t stream, int delta_dtype, const flo
   TA_REQUIRE(mx_on(x, 16) && mx_on(delta, 16) && mx_on(bias, 16) && mx_on(weight, 16) && mx_on(to, 16) && mx_on(codes, 16),
              "ta_add_rmsnorm_mx8: rows do not start on 16 bytes");
   TA_REQUIRE(to || (planes == 0 && !bias), "ta_add_rmsnorm_mx8: what is added goes nowhere");
-  if (n == 0) return 0;
-  if (delta_dtype == TA_F32)
-    launch_norm<float>(stream, x, (const float*)delta, planes, bias, weight, eps, to, (uint8_t*)codes, (uint8_t*)scales, n, d);
-  else
-    launch_norm<bf16_t>(stream, x, (const bf16_t*)delta, planes, bias, weight, eps, to, (uint8_t*)codes, (uint8_t*)scales, n, d);
-  return ta_check_launch("ta_add_rmsnorm_mx8");
+  // a launch has fewer than 2^32 threads, and a row has up to 1,024 of them
+  const long long most = 1 << 21, plane = (long long)n * d;
+  for (long long at = 0; at < n; at += most) {
+    const int rows = (int)(n - at < most ? n - at : most);
+    const long long from = at * d;
+    uint8_t *c = (uint8_t*)codes + from, *s = (uint8_t*)scales + from / MX_BLOCK;
+    float* sum = to ? to + from : nullptr;
+    if (delta_dtype == TA_F32)
+      launch_norm<float>(stream, x + from, delta ? (const float*)delta + from : nullptr, planes, bias, weight, eps, sum, c, s, rows, d, plane);
+    else
+      launch_norm<bf16_t>(stream, x + from, delta ? (const bf16_t*)delta + from : nullptr, planes, bias, weight, eps, sum, c, s, rows, d, plane);
+    if (ta_check_launch("ta_add_rmsnorm_mx8")) return 1;
+  }
+  return 0;
 }
