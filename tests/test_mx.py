@@ -120,3 +120,26 @@ def test_a_k_beyond_a_launchs_integers_is_refused(k, monkeypatch):
                  lambda: kernels.gemm_mx4_scratch(True, False, 64, k, 4096)):
         with pytest.raises(kernels.KernelError, match="fewer than 2\\^31"):
             call()
+
+
+def test_columns_beyond_a_launchs_threads_are_refused():
+    """A launch counts its threads in 32 bits: what is beyond them is refused by name, and nothing on the way there overflows."""
+    lib = kernels.library()
+    for kw in (dict(M=1, N=1 << 30, K=32), dict(M=1, N=2147483647, K=32), dict(M=16, N=2147483647, K=512), dict(M=1, N=1 << 30, K=512),
+               dict(M=40, N=2147483647, K=512, scratch=AT, room=1 << 62)):
+        _refused(_gemm(lib, **kw), b"ta_gemm_mx4:")
+        assert b"more than a launch holds" in lib.ta_last_error()
+        _refused(_gemm8(lib, **kw), b"ta_gemm_mx4_mx8:")
+        assert b"more than a launch holds" in lib.ta_last_error()
+    for kw in (dict(M=4, N=0x3fffffff, K=512, glu=1), dict(M=1, N=0x3fffffff, K=32, glu=1)):
+        _refused(_gemm(lib, **kw), b"ta_gemm_mx4:")
+        assert b"more than a launch holds" in lib.ta_last_error()
+
+
+def test_what_a_launch_still_holds_goes_out():
+    if torch.cuda.is_available():
+        pytest.skip("the operands are addresses of nothing: only where no kernel can be launched")
+    lib = kernels.library()
+    for call, kw in ((_gemm, dict(M=1, N=(1 << 30) - 16, K=32)), (_gemm8, dict(M=8, N=(1 << 30) - 16, K=32)), (_gemm8, dict(M=2147483647, N=1, K=32)),
+                     (_gemm8, dict(M=2147483647, N=130, K=4096, scratch=AT, room=1 << 62))):
+        assert call(lib, **kw) != 0 and b"no ROCm-capable device" in lib.ta_last_error(), lib.ta_last_error()

@@ -502,6 +502,22 @@ def test_more_elements_than_32_bits_count():
     _check_rows(kernels.Mx8(rows.codes[m - 1:], rows.scales[m - 1:]), v, 2.0 ** -42)
 
 
+def test_products_of_more_rows_than_a_launch_has_threads_for():
+    """2^29 rows are 2^23 tiles of 512 threads: rows on both sides of the launches' borders, every 2^26 rows, and the last."""
+    m, n, k = 2 ** 29 + 70, 3, 32
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("wants 24 GB")
+    w = _weights(n, k, 24)
+    x = kernels.Mx8.empty(m, k, DEV)
+    _bits(x.codes).random_(0, 127, generator=_gen(24))                                 # any positive value
+    x.scales.random_(120, 130, generator=_gen(25))
+    y = kernels.gemm_mx4(x, w, torch.full((m, n), float("nan"), device=DEV, dtype=torch.bfloat16))
+    assert bool(y.isfinite().all())
+    for at in (0, 2 ** 26 - 40, 5 * 2 ** 26 - 40, 2 ** 29 - 40, m - 80):
+        part = slice(at, at + 80)
+        _close(y[part], U.values8(x.codes[part], x.scales[part]), U.values4(w.codes, w.scales), ALIGNED)
+
+
 # ------------------------------------------------------------------ refusals
 def test_nothing_to_do():
     w = _weights(40, 64)

@@ -287,11 +287,16 @@ __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
 }
 
 #define MX_LDS (160 * 1024)
+// A launch counts its threads in 32 bits and loses what is beyond without an error. Rows that would be too many go out in several launches
+// (MX_ROWS), columns are refused.
+#define MX_ROWS (1 << 26)
+static bool mx_launch_holds(long long groups, int threads) { return groups * threads <= 0xffffffffLL; }
+
 template <bool X8, bool GLU, int S, int R, int T = 1>
 static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) {
   constexpr int x = R * (X8 ? 8 : 16) * S * 16, sums = (GLU ? 2 : T) * 1024;
   const auto kernel = mx_few_kernel<X8, GLU, S, R, T>;
-  const int chunks = g.K / (128 * S), grid = (g.N + 16 * T - 1) / (16 * T);
+  const int chunks = g.K / (128 * S), grid = (int)(((long long)g.N + 16 * T - 1) / (16 * T));
   // as many waves as give every CU 16, then the fewest that need as many turns; one buffer of x does for one turn
   int waves = (16 * 256 + grid - 1) / grid;
   waves = waves < 4 ? 4 : waves > 16 ? 16 : waves;
@@ -304,6 +309,7 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
   }
   const int turns = (chunks + waves - 1) / waves;
   if (turns > 0) waves = (chunks + turns - 1) / turns;
+  TA_REQUIRE(mx_launch_holds(grid, waves * 64), "%s: M=%d N=%d are more than a launch holds", what, g.M, g.N);
   static int allowed = 64 * 1024;
   if (waves * bytes > allowed) {
     const hipError_t e =
@@ -758,8 +764,8 @@ static int mx_tile_launch(const char* what, hipStream_t stream, const MxGemm& g,
     if (e != hipSuccess) return ta_fail("%s: %d bytes of LDS refused (%s)", what, most, hipGetErrorString(e));
     asked = true;
   }
-  z.m_tiles = (g.M + BM - 1) / BM;
-  z.n_tiles = (g.N + (GLU ? BN / 2 : BN) - 1) / (GLU ? BN / 2 : BN);
+  z.m_tiles = (int)(((long long)g.M + BM - 1) / BM);
+  z.n_tiles = (int)(((long long)g.N + (GLU ? BN / 2 : BN) - 1) / (GLU ? BN / 2 : BN));
   kernel<<<z.m_tiles * z.n_tiles * z.parts, 512, bytes, stream>>>(g, z);
   return ta_check_launch(what);
 }
@@ -815,12 +821,17 @@ static int mx_tiles(const char* what, hipStream_t stream, const MxGemm& g, void*
   TA_REQUIRE(plan.bytes == 0 || (scratch && scratch_bytes >= plan.bytes && (uintptr_t)scratch % 16 == 0),
              "%s: %lld bytes of scratch, %lld are needed", what, scratch ? scratch_bytes : 0LL, plan.bytes);
   TA_REQUIRE((rows + 256) * (g.K / 2) <= 0xffffffffLL || !GLU, "%s: gates and ups of %d x %d lie more than 4 GB apart", what, g.N, g.K);
+  // all launches of the call, before the first
+  const auto& form = mx_forms[plan.form];
+  const long long xrows = X8 ? g.M : 0, tiles = ((long long)g.M + form.bm - 1) / form.bm * ((rows + form.bn - 1) / form.bn),
+                  scales_grid = plan.scales ? ((xrows + rows) * mx_step(g.K) / 4 + 255) / 256 : 0,
+                  planes_grid = plan.parts > 1 ? ((long long)g.M * (((long long)g.N + 3) / 4) + 255) / 256 : 0;
+  TA_REQUIRE(mx_launch_holds(tiles * plan.parts, 512) && mx_launch_holds(scales_grid, 256) && mx_launch_holds(planes_grid, 256),
+             "%s: M=%d N=%d are more than a launch holds", what, g.M, g.N);
   MxTiles z = {g.xs, g.scales, g.K % 512 == 0 && aligned ? g.K / MX_BLOCK : 0, 0, 0, plan.parts, plan.part_steps, nullptr};
   if (plan.scales) {
     z.step = mx_step(g.K);
-    const long long xrows = X8 ? g.M : 0, grid = ((xrows + rows) * z.step / 4 + 255) / 256;
-    TA_REQUIRE(grid <= 0x7fffffffLL, "%s: M=%d N=%d K=%d: more scales than a launch holds", what, g.M, g.N, g.K);
-    mx_scales_kernel<<<(int)grid, 256, 0, stream>>>(g.xs, g.scales, (uint8_t*)scratch, xrows, xrows + rows, g.K / MX_BLOCK, z.step);
+    mx_scales_kernel<<<(int)scales_grid, 256, 0, stream>>>(g.xs, g.scales, (uint8_t*)scratch, xrows, xrows + rows, g.K / MX_BLOCK, z.step);
     if (ta_check_launch(what)) return 1;
     z.xs = (const uint8_t*)scratch;
     z.ws = z.xs + (size_t)xrows * z.step;
@@ -833,9 +844,7 @@ static int mx_tiles(const char* what, hipStream_t stream, const MxGemm& g, void*
   else if (plan.form == 2) rc = mx_tile_launch<true, false, 128, 256, 2, 4, 1, 3>(what, stream, g, z);
   else rc = mx_tile_launch<true, false, 256, 256, 2, 4, 1, 3>(what, stream, g, z);
   if (rc || plan.parts == 1) return rc;
-  const long long grid = ((long long)g.M * ((g.N + 3) / 4) + 255) / 256;
-  TA_REQUIRE(grid <= 0x7fffffffLL, "%s: M=%d N=%d are more than a launch holds", what, g.M, g.N);
-  mx_planes_kernel<GLU><<<(int)grid, 256, 0, stream>>>(g, z.planes, plan.parts);
+  mx_planes_kernel<GLU><<<(int)planes_grid, 256, 0, stream>>>(g, z.planes, plan.parts);
   return ta_check_launch(what);
 }
 
@@ -879,6 +888,10 @@ static bool mx_few(bool x8, bool glu, int M, int N, int K, bool aligned) {
 
 // Bytes of scratch for M rows in 8 bits (x8) or bfloat16; aligned: all scales start on 16 bytes.
 extern "C" long long ta_gemm_mx4_scratch(int x8, int swiglu, int M, int N, int K, int aligned) {
+  if (M > MX_ROWS) {
+    const long long first = ta_gemm_mx4_scratch(x8, swiglu, MX_ROWS, N, K, aligned), last = ta_gemm_mx4_scratch(x8, swiglu, M % MX_ROWS, N, K, aligned);
+    return first > last ? first : last;
+  }
   if (M <= 0 || N <= 0 || K < MX_BLOCK || mx_few(x8, swiglu, M, N, K, aligned)) return 0;
   return mx_plan(x8, swiglu, M, N, K, aligned).bytes;
 }
@@ -917,15 +930,9 @@ extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const 
   return mx_few_launch<false, false, 2, 16>(what, stream, g);
 }
 
-// 8-bit rows, codes [M][K] and bytes [M][K/32]; out bfloat16. scratch: ta_gemm_mx4_scratch bytes on 16.
-extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs, const void* codes, const void* scales, const float* bias,
-                               void* out, long long ldo, int M, int N, int K, void* scratch, long long scratch_bytes) {
-  static const char what[] = "ta_gemm_mx4_mx8";
-  const MxGemm g = {x, (const uint8_t*)xs, (const uint8_t*)codes, (const uint8_t*)scales, bias, out, K, ldo, M, N, K, 0};
-  if (mx_gemm_check(what, g)) return 1;
-  TA_REQUIRE(K <= 1 << 23, "%s: k %d: at most 8,388,608", what, K);         // 256 rows within 31 bits
-  if (M == 0) return 0;
-  if (!mx_few(true, false, M, N, K, ((uintptr_t)xs | (uintptr_t)scales) % 16 == 0))
+static int mx_product8(const char* what, hipStream_t stream, const MxGemm& g, void* scratch, long long scratch_bytes) {
+  const int M = g.M, N = g.N, K = g.K;
+  if (!mx_few(true, false, M, N, K, ((uintptr_t)g.xs | (uintptr_t)g.scales) % 16 == 0))
     return mx_tiles<true, false>(what, stream, g, scratch, scratch_bytes);
   // (1 x 28,672 x 4,096 in chunks of 512 11.8 us, of 256 14.9; 16 rows 21.7 and 20.9)
   if (M <= 1) return mx_few_launch<true, false, 4, 1>(what, stream, g);
@@ -934,4 +941,22 @@ extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs
     return M <= 8 ? mx_few_launch<true, false, 2, 8, 2>(what, stream, g) : mx_few_launch<true, false, 2, 16, 2>(what, stream, g);
   if (M <= 8) return mx_few_launch<true, false, 2, 8>(what, stream, g);
   return mx_few_launch<true, false, 2, 16>(what, stream, g);
+}
+
+// 8-bit rows, codes [M][K] and bytes [M][K/32]; out bfloat16. scratch: ta_gemm_mx4_scratch bytes on 16.
+extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs, const void* codes, const void* scales, const float* bias,
+                               void* out, long long ldo, int M, int N, int K, void* scratch, long long scratch_bytes) {
+  static const char what[] = "ta_gemm_mx4_mx8";
+  const MxGemm g = {x, (const uint8_t*)xs, (const uint8_t*)codes, (const uint8_t*)scales, bias, out, K, ldo, M, N, K, 0};
+  if (mx_gemm_check(what, g)) return 1;
+  TA_REQUIRE(K <= 1 << 23, "%s: k %d: at most 8,388,608", what, K);         // 256 rows within 31 bits
+  for (long long at = 0; at < M; at += MX_ROWS) {
+    MxGemm part = g;
+    part.x = (const uint8_t*)x + at * K;
+    part.xs = g.xs + at * (K / MX_BLOCK);
+    part.out = (uint8_t*)out + at * ldo * 2;
+    part.M = (int)(M - at < MX_ROWS ? M - at : MX_ROWS);
+    if (mx_product8(what, stream, part, scratch, scratch_bytes)) return 1;
+  }
+  return 0;
 }
