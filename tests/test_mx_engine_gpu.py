@@ -98,6 +98,36 @@ def test_logits_with_rows_in_8_bits(name, lens, graphs):
         assert _off(g, plain.forward(q)[n - 1:]) < 0.08
 
 
+@pytest.mark.parametrize("activations", [None, "mx8"])
+def test_steps_of_more_sequences_than_the_few_rows_products_take(activations):
+    """70 sequences, a recorded step of 96 rows: with bfloat16 rows every product widens its weights inside the recording. Replayed, and between
+    replays a prompt that uses the same scratch eagerly."""
+    model, plain = _model("D", activations)
+    count, decode = 70, 5
+    got = {}
+    for graphs in (False, True):
+        model.use_graphs = graphs
+        cache = model.new_cache(64 * (count + 4), count + 2)
+        seqs = [G.tokens("D", 2 + i % 3 + decode, 400 + i) for i in range(count)]
+        slots = [cache.alloc_slot() for _ in seqs]
+        model.step(cache, [ta.Entry(s, q[:-decode], want=[]) for s, q in zip(slots, seqs)])
+        out = []
+        for t in range(decode):
+            out.append(model.step(cache, [ta.Entry(s, [q[len(q) - decode + t]], want=[0]) for s, q in zip(slots, seqs)]).clone())
+            other = cache.alloc_slot()
+            model.step(cache, [ta.Entry(other, G.tokens("D", 90, 7), want=[89])])
+            cache.free_slot(other)
+        assert bool(cache.graphs) == graphs and not cache.graphs_failed
+        got[graphs] = torch.stack(out, 1).double().cpu().numpy()
+    for graphs in (False, True):
+        for i in (0, 1, 34, 63, 64, 69):
+            want = plain.forward(seqs[i])[-decode:]
+            if activations:
+                assert _off(got[graphs][i], want) < 0.08
+            else:
+                assert np.abs(want - got[graphs][i]).max() < G.TOL["bfloat16"]
+
+
 def test_generates_and_holds_fewer_bytes():
     folder = G.folder("E", "bfloat16")
     wide = G.engine("E", "bfloat16")

@@ -145,6 +145,8 @@ def test_norm_of_more_rows_than_a_launch_has_threads_for():
         y = x[part].double() + delta[0, part].double() + delta[1, part].double()
         y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + 1e-5) * w.double()
         _check_rows(kernels.Mx8(out.codes[part], out.scales[part]), y, 2.0 ** -42)
+    del x, delta, out, stream
+    torch.cuda.empty_cache()
 
 
 def test_norm_of_rows_that_hold_what_is_not_finite():
@@ -407,6 +409,27 @@ def test_scales_at_the_ends_of_their_range(m, eight):
         _close(got[:, ~over], U.values8(a.codes, a.scales) if eight else a.double(), w64[~over], ALIGNED if eight else 0.0)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("n,k", [(33, 64), (33, 1056), (9000, 2048)])
+@pytest.mark.parametrize("m", [1, 8, 20, 40, 64, 100])
+def test_products_under_the_smallest_and_the_largest_scale(m, n, k, eight):
+    """The scale bytes 0, whose power of two is no normal float32, and 254, in every kernel; under 254 codes of less than 2, as bfloat16 holds
+    nothing of 2^128 and more."""
+    if not eight and m > kernels.MX4_MAX_ROWS:
+        pytest.skip("bfloat16 rows go up to 64")
+    g = _gen(m, n, k)
+    small = torch.tensor([c for c in range(16) if c % 8 < 4], dtype=torch.uint8, device=DEV)         # 0, 0.5, 1, 1.5 and their negatives
+    for byte, e in ((0, 100), (254, -100)):
+        half = [small[torch.randint(0, 8, (n, k // 2), generator=g, device=DEV)] if byte else
+                torch.randint(0, 16, (n, k // 2), generator=g, device=DEV, dtype=torch.uint8) for _ in range(2)]
+        w = kernels.Mx4(half[0] | half[1] << 4, torch.full((n, k // 32), byte, dtype=torch.uint8, device=DEV))
+        x = torch.randn(m, k, generator=g, device=DEV) * 2.0 ** e
+        a = kernels.mx8_pack(x, kernels.Mx8.empty(m, k, DEV)) if eight else x.bfloat16()
+        got = kernels.gemm_mx4(a, w, torch.empty(m, n, device=DEV, dtype=torch.bfloat16))
+        assert bool((got != 0).any()) and bool(got.isfinite().all())
+        _close(got, U.values8(a.codes, a.scales) if eight else a.double(), U.values4(w.codes, w.scales), ALIGNED if eight else 0.0)
+
+
 def test_chain_captured_replayed_and_on_another_stream():
     """Norm, product, activation, product on 8-bit rows, and the gated product on bfloat16 rows: eager, recorded and replayed between other
     work, and on a stream of its own; every time the same bits."""
@@ -503,19 +526,21 @@ def test_more_elements_than_32_bits_count():
 
 
 def test_products_of_more_rows_than_a_launch_has_threads_for():
-    """2^29 rows are 2^23 tiles of 512 threads: rows on both sides of the launches' borders, every 2^26 rows, and the last."""
-    m, n, k = 2 ** 29 + 70, 3, 32
-    if torch.cuda.mem_get_info()[0] < 40e9:
-        pytest.skip("wants 24 GB")
+    """2^30 rows are 2^23 tiles of 512 threads: rows on both sides of the launches' borders, every 2^26 rows, and the last."""
+    m, n, k = 2 ** 30 + 70, 3, 32
+    if torch.cuda.mem_get_info()[0] < 70e9:
+        pytest.skip("wants 50 GB")
     w = _weights(n, k, 24)
     x = kernels.Mx8.empty(m, k, DEV)
     _bits(x.codes).random_(0, 127, generator=_gen(24))                                 # any positive value
     x.scales.random_(120, 130, generator=_gen(25))
     y = kernels.gemm_mx4(x, w, torch.full((m, n), float("nan"), device=DEV, dtype=torch.bfloat16))
     assert bool(y.isfinite().all())
-    for at in (0, 2 ** 26 - 40, 5 * 2 ** 26 - 40, 2 ** 29 - 40, m - 80):
+    for at in (0, 2 ** 26 - 40, 5 * 2 ** 26 - 40, 2 ** 30 - 40, m - 80):
         part = slice(at, at + 80)
         _close(y[part], U.values8(x.codes[part], x.scales[part]), U.values4(w.codes, w.scales), ALIGNED)
+    del x, y
+    torch.cuda.empty_cache()
 
 
 # ------------------------------------------------------------------ refusals
