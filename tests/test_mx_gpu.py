@@ -282,6 +282,25 @@ def test_products_of_many_8_bit_rows(m, n, k):
     _close(got, U.values8(x.codes, x.scales), U.values4(w.codes, w.scales), ALIGNED)
 
 
+@pytest.mark.parametrize("m", [16, 17, 63, 64])
+def test_gated_products_whose_gates_and_ups_lie_more_than_4_gb_apart(m):
+    n, k = 2 ** 23 + 70, 512
+    if torch.cuda.mem_get_info()[0] < 20e9:
+        pytest.skip("wants 10 GB")
+    w = kernels.Mx4.empty(2 * n, k, DEV)
+    w.codes.random_(0, 256, generator=_gen(26))
+    w.scales.random_(118, 124, generator=_gen(27))
+    x, bias = _randn(m, k, key=(26,)).bfloat16(), _randn(2 * n, key=(26,))
+    out = torch.full((m, n), float("nan"), device=DEV, dtype=torch.bfloat16)
+    kernels.gemm_mx4(x, w, out, bias, swiglu=True)
+    assert not bool(out.isnan().any())
+    for at in (0, 2 ** 23 - 150, n - 200):          # (ending at n at most)
+        cols = torch.cat((torch.arange(at, at + 200, device=DEV), torch.arange(n + at, n + at + 200, device=DEV)))
+        _close(out[:, at:at + 200], x.double(), U.values4(w.codes[cols], w.scales[cols]), 0.0, True, bias[cols])
+    del w, out
+    torch.cuda.empty_cache()
+
+
 # more weights than groups of 16 rows pay for, in one part of k and in several; k off a step, off a load of scales, and with more
 # scales than LDS holds
 @pytest.mark.parametrize("n,k", [(8209, 4096), (4100, 14336), (7001, 5152), (33000, 1056), (33000, 8224)])

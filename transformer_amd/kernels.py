@@ -3109,9 +3109,9 @@ def gemm_mx4_scratch(eight: bool, swiglu: bool, rows: int, n: int, k: int, align
 MX_FEW_ROWS = 16        # rows up to which no call needs any
 
 
-
 def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, swiglu: bool = False) -> torch.Tensor:
-    """out = a @ w.T (+ bias) with 4-bit weights, sums in float32.
+    """out = a @ w.T (+ bias) with 4-bit weights, sums in float32. k up to 8,388,608, rows of a bfloat16 ``a`` up to 16,777,216 values
+    apart, as many columns as one launch has threads for (below 2^30).
 
     a bfloat16, at most ``MX4_MAX_ROWS`` rows (more: ``mx4_unpack`` and a product of many bfloat16 rows): the weights enter with
     their exact values (one of 2^128 and more, which bfloat16 does not hold, as an infinity), out float32 or bfloat16. swiglu: w
@@ -3148,6 +3148,11 @@ def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, 
         return out
     if (m | n | k) >> 31:
         _too_large("gemm_mx4", rows=m, n=n, k=k)
+    if swiglu and MX_FEW_ROWS < m <= MX4_MAX_ROWS and (n + 256) * (k // 2) >> 32:
+        # a tile counts from its gates to their ups in 32 bits: rows in the groups whose kernel has an address for either
+        for first in range(0, m, MX_FEW_ROWS):
+            gemm_mx4(a[first:first + MX_FEW_ROWS], w, out[first:first + MX_FEW_ROWS], bias, True)
+        return out
     xs, ws = a.scales.data_ptr() if eight else 0, w.scales.data_ptr()
     scratch = need = 0
     if m > MX_FEW_ROWS:
