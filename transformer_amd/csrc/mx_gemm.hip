@@ -5,9 +5,14 @@
 // float32 sums.
 //
 // 8-bit rows: v_mfma_scale_f32_16x16x128_f8f6f4 takes both operands and both scales as they are. It lines up the 128 products
-// of a call to the largest one's exponent before it adds them, which leaves some 15 bits below it (measured: 5e-5 of the sum
-// of magnitudes where the operands' exponents fill their range); results are therefore bfloat16, which rounds 80 times as
-// coarsely, and only the running sums over k are float32.
+// of a call to the largest one's exponent before it adds them, which leaves some 15 bits below it; from call to call sums are
+// float32. Measured on normal weights and normed rows (64 x 4,096 over k = 14,336): the sums are off by 6.8e-6 of the root of their
+// products' sum of squares (5e-5 at most, no bias), where float32 sums are off by 4e-8. Beside a result's size that is some 1/240 of
+// bfloat16's rounding, 1.65e-3: 0.6 % of the results round to the neighbour, and the results as a whole are as far from 64 bits
+// as rounded float32 sums are, 1.6536e-3. So they leave as bfloat16 only; one result in 500, which cancels to little beside its
+// products, is off by more than a bfloat16's half step of itself (as it is, by far more, from the rows' rounding to 4 bits).
+//
+// Times below are GPU time a call inside a graph, weights out of memory; two forms compared were measured in turn.
 #include "mx.h"
 
 __device__ __forceinline__ mx_bf16x8 mx_widen8(uint32_t codes, float scale) {
@@ -34,8 +39,8 @@ struct MxGemm {
   int wide;                   // out is float32, else bfloat16
 };
 
-// Results go out in wide stores whatever the row's length leaves of their alignment (1,638 x 2,518 over k = 704, rows on 4 bytes, 12.4 us;
-// 16.3 a row at a time through LDS, 29 single)
+// Results go out in wide stores whatever the row's length leaves of their alignment (1,638 x 2,518 over k = 704, rows on 4 bytes, with operands
+// in the caches 12.4 us; 16.3 a row at a time through LDS, 29 single)
 typedef mx_f32x4 mx_f32x4_any __attribute__((aligned(4)));
 typedef mx_u32x4 mx_u32x4_any __attribute__((aligned(2)));
 typedef mx_u32x2 mx_u32x2_any __attribute__((aligned(2)));
@@ -87,11 +92,12 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, long long at, const fl
 // behind the whole chunks is one wave's, with loads that ask where k ends.
 //
 // Waves: every CU wants some 16 of them with two chunks each on their way, which 64 KB of weights in flight keep the memory
-// busy with; fewer than four a workgroup leave too many of the sums' exchanges.
+// busy with; fewer than four a workgroup leave too many of the sums' exchanges. LDS may hold fewer: 8 bfloat16 rows in chunks of 512
+// take 16 KB a wave, so ten.
 //
-// Measured (GPU time): 8-bit rows, 1 x 28,672 x 4,096 12.9 us (4.8 TB/s of a copy's 5.1), 8 x 14,336 x 4,096 9.7, 16 rows 10.8, where x
-// through LDS costs as much as the weights; bfloat16 rows 1 x 4,096 x 4,096 4.7 (launch, one way to memory, the sums), 1 x 4,096 x 14,336
-// 8.7, 8 x 4,096 x 14,336 10.5, gated 1 x 14,336 x 4,096 16.2 (3.9 TB/s: an instruction for every two codes).
+// Measured: 8-bit rows, 1 x 28,672 x 4,096 12.6 us (5.0 TB/s of a copy's 5.1), 8 x 14,336 x 4,096 10.7, 16 rows 11.3, where x
+// through LDS costs as much as the weights; bfloat16 rows 1 x 4,096 x 4,096 4.6 (launch, one way to memory, the sums), 1 x 4,096 x 14,336
+// 8.4, 8 x 4,096 x 14,336 11.8, gated 1 x 14,336 x 4,096 15.4 (4.1 TB/s: an instruction for every two codes).
 template <bool X8, bool GLU, int S, int R, int T>
 __global__ __launch_bounds__(1024) void mx_few_kernel(MxGemm g, int bytes) {
   if (gridDim.y > 1) {                          // this workgroup's R rows
@@ -335,9 +341,12 @@ static int mx_few_launch(const char* what, hipStream_t stream, const MxGemm& g) 
 //
 // The weights are the first operand: a lane then holds 4 neighbouring columns of one row. Row p of the tile t of 16 stands for
 // column 16 (p / 4) + 4 t + p % 4 of the wave's 64, so a lane's four tiles are 16 neighbouring columns, stored 16 bytes at a time.
-// Pieces of 16 bytes are permuted by the row's number, so that sixteen lanes' reads meet no bank twice.
-// Measured: a step of 64 x 128 takes 0.33 us, of 256 x 256 1.6, where the matrix instructions alone need 0.13 and 1.0, the way into LDS 0.11
-// and 0.33 and the reads 0.11 and 0.5; 4,096 x 28,672 x 4,096 388 us (2.5 PFLOP/s of the instruction's 4.2), 512 x 4,096 x 14,336 39.
+// Pieces of 16 bytes are permuted by the row's number, so that the addresses of sixteen lanes (one q) meet every bank once. The counters
+// still have 1.25 cycles of bank conflicts for each LDS instruction of the 256 x 256 tile, of 4.5 that it takes; what they come from is
+// not known.
+// Measured: a step of 64 x 128 takes 0.33 us with operands in the caches (0.45 out of memory), of 256 x 256 1.6, where the matrix
+// instructions alone need 0.13 and 1.0, the way into LDS 0.11 and 0.33 and the reads 0.11 and 0.5: the small tile's parts add up and do not
+// overlap. 4,096 x 28,672 x 4,096 375 us (2.6 PFLOP/s of the instruction's 4.2), 512 x 4,096 x 14,336 50 (38 to 42 in the caches).
 // Where the tiles do not fill the CUs, k is cut among `parts` workgroups, which leave float32 sums in planes; mx_planes_kernel adds
 // them in order and finishes. GLU: a tile holds 64 gates and their 64 ups, a lane's 16 columns are then 8 of either.
 __device__ __host__ __forceinline__ long long mx_pad(int n) { return (n + 3LL) / 4 * 4; }
@@ -354,7 +363,7 @@ __device__ __forceinline__ void mx_to_lds16(const void* base, uint32_t offset, u
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(lds) : "m0", "memory");
 }
 
-// which of a row's pieces lie where: sixteen rows' reads of a piece meet every bank once, two rows of 8 pieces (of 256 bytes
+// which of a row's pieces lie where: sixteen rows' addresses of a piece have every bank once, two rows of 8 pieces (of 256 bytes
 // together) or one of 16 in each of the places that a bank has
 template <bool X8>
 __device__ __forceinline__ uint32_t mx_flip(uint32_t row) {
@@ -779,7 +788,8 @@ struct MxPlan {
   double us;
 };
 // Tiles and what 128 k of one take while every CU has one (measured on MI355X in us: k 4,096 and 14,336, one to seven
-// rounds)
+// rounds, with the start and the end of a tile spread over its steps). Of 17 shapes the choice is the fastest of all forms and cuts, or within
+// 2 %, for 16; 128 x 6,144 over k = 4,096 takes 16.4 us in two parts and 14.0 in one.
 static const struct {
   int bm, bn;
   double us;
@@ -914,8 +924,9 @@ extern "C" int ta_gemm_mx4(hipStream_t stream, int out_dtype, int swiglu, const 
   if (M == 0) return 0;
   if (!mx_few(false, swiglu, M, N, K, (uintptr_t)scales % 16 == 0))
     return swiglu ? mx_tiles<false, true>(what, stream, g, scratch, scratch_bytes) : mx_tiles<false, false>(what, stream, g, scratch, scratch_bytes);
-  // chunks of 512 where registers allow (1 x 4,096 x 14,336 7.6 us, with 256 8.4); with ups beside the gates 256 (14.9 and 19.3), as with 16
-  // rows, whose LDS leaves a CU fewer waves (16 x 14,336 x 4,096 14.6 and 17.6). Fewer rows brought: 1 x 4,096 x 14,336 with room for 16 10.7
+  // chunks of 512 where registers allow (1 x 4,096 x 14,336 8.4 us, with 256 8.9); with ups beside the gates 256 (1 x 14,336 x 4,096 15.4, with
+  // 512 20.1), as with 16 rows, whose LDS leaves a CU fewer waves (16 x 14,336 x 4,096 14.5 and 17.9). Fewer rows brought: 1 x 4,096 x 14,336
+  // with room for 16 12.1
   if (swiglu) {
     if (M <= 1) return mx_few_launch<false, true, 2, 1>(what, stream, g);
     if (M <= 4) return mx_few_launch<false, true, 2, 4>(what, stream, g);
@@ -934,7 +945,7 @@ static int mx_product8(const char* what, hipStream_t stream, const MxGemm& g, vo
   const int M = g.M, N = g.N, K = g.K;
   if (!mx_few(true, false, M, N, K, ((uintptr_t)g.xs | (uintptr_t)g.scales) % 16 == 0))
     return mx_tiles<true, false>(what, stream, g, scratch, scratch_bytes);
-  // (1 x 28,672 x 4,096 in chunks of 512 11.8 us, of 256 14.9; 16 rows 21.7 and 20.9)
+  // (1 x 28,672 x 4,096 in chunks of 512 12.6 us, of 256 14.2; 16 rows 51 and 20.1)
   if (M <= 1) return mx_few_launch<true, false, 4, 1>(what, stream, g);
   if (M <= 4) return mx_few_launch<true, false, 4, 4>(what, stream, g);
   if (mx_few_pairs(true, M, N, K))

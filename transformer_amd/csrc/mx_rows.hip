@@ -312,8 +312,8 @@ template <typename TD>
 static void launch_norm(hipStream_t stream, const float* x, const TD* delta, int planes, const float* bias, const float* weight, float eps,
                         float* to, uint8_t* codes, uint8_t* scales, int n, int d, long long plane) {
 #define MX_NORM(T, H) add_rmsnorm_mx8_kernel<TD, T, H><<<n, T, 0, stream>>>(x, delta, plane, planes, bias, weight, eps, to, codes, scales, d, 1. / d)
-  // as many threads as a row has pieces: 8 x 8,192 3.9 us (with 512 threads of two pieces 4.4), 2,048 x 8,192 39.8 (40.6), 2,048 x 4,096
-  // 22.2 (with 256 threads of two 23.3)
+  // as many threads as a row has pieces: out of memory 8 x 8,192 4.1 us (with 512 threads of two pieces 5.2), 2,048 x 8,192 42.3 (42.9), 2,048 x
+  // 4,096 22.1 (with 256 threads of two 23.0)
   if (d <= 2048) MX_NORM(256, 1);
   else if (d <= 4096) MX_NORM(512, 1);
   else if (d <= 8192) MX_NORM(1024, 1);
