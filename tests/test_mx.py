@@ -136,6 +136,16 @@ def test_columns_beyond_a_launchs_threads_are_refused():
         assert b"more than a launch holds" in lib.ta_last_error()
 
 
+def test_rows_of_several_launches_have_their_scratch_checked_before_the_first():
+    """2^26 rows need none here, the 100 behind them planes."""
+    lib, rows = kernels.library(), (1 << 26) + 100
+    need = kernels.gemm_mx4_scratch(True, False, rows, 512, 2048)
+    assert kernels.gemm_mx4_scratch(True, False, 1 << 26, 512, 2048) == 0 < need == kernels.gemm_mx4_scratch(True, False, 100, 512, 2048)
+    for kw in (dict(), dict(scratch=AT, room=need - 1), dict(scratch=c_void_p((1 << 20) + 8), room=need)):
+        _refused(_gemm8(lib, M=rows, N=512, K=2048, **kw), b"ta_gemm_mx4_mx8:")
+        assert b"scratch" in lib.ta_last_error()
+
+
 def test_what_a_launch_still_holds_goes_out():
     if torch.cuda.is_available():
         pytest.skip("the operands are addresses of nothing: only where no kernel can be launched")

@@ -961,6 +961,11 @@ extern "C" int ta_gemm_mx4_mx8(hipStream_t stream, const void* x, const void* xs
   const MxGemm g = {x, (const uint8_t*)xs, (const uint8_t*)codes, (const uint8_t*)scales, bias, out, K, ldo, M, N, K, 0};
   if (mx_gemm_check(what, g)) return 1;
   TA_REQUIRE(K <= 1 << 23, "%s: k %d: at most 8,388,608", what, K);         // 256 rows within 31 bits
+  if (M > MX_ROWS) {                            // before the first launch: the last may need more than it
+    const long long need = ta_gemm_mx4_scratch(1, 0, M, N, K, ((uintptr_t)xs | (uintptr_t)scales) % 16 == 0);
+    TA_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && (uintptr_t)scratch % 16 == 0), "%s: %lld bytes of scratch, %lld are needed", what,
+               scratch ? scratch_bytes : 0LL, need);
+  }
   for (long long at = 0; at < M; at += MX_ROWS) {
     MxGemm part = g;
     part.x = (const uint8_t*)x + at * K;
