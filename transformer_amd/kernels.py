@@ -2884,7 +2884,7 @@ _MX_TYPES = {
     "ta_mx8_pack": (_p, _i, _p, _l, _p, _p, _l, _i),
     "ta_swiglu_mx8": (_p, _i, _p, _l, _p, _p, _p, _l, _i),
     "ta_add_rmsnorm_mx8": (_p, _i, _p, _p, _i, _p, _p, c_float, _p, _p, _p, _i, _i),
-    "ta_gemm_mx4": (_p, _i, _i, _p, _l, _p, _p, _p, _p, _l, _i, _i, _i),
+    "ta_gemm_mx4": (_p, _i, _i, _p, _l, _p, _p, _p, _p, _l, _i, _i, _i, _p, _l),
     "ta_gemm_mx4_mx8": (_p, _p, _p, _p, _p, _p, _p, _l, _i, _i, _i, _p, _l),
 }
 _mx_ready = {}
@@ -2905,6 +2905,10 @@ def _here(what: str, *tensors):
     for t in tensors:
         if t is not None and t.get_device() != at:
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{at}")
+
+
+def _too_large(what: str, **sizes):
+    raise KernelError(f"{what}: {', '.join(f'{n} {v}' for n, v in sizes.items())}: a launch counts each in 32 bits, fewer than 2^31")
 
 
 def _vector(t: Optional[torch.Tensor], n: int, at: int) -> bool:
@@ -2987,6 +2991,8 @@ def mx4_pack(w: torch.Tensor, out: Mx4) -> Mx4:
     if tuple(w.shape) != out.shape:
         raise KernelError(f"mx4_pack: w {tuple(w.shape)} out {out.shape}")
     _here("mx4_pack", w, out.codes)
+    if w.shape[1] >> 31:
+        _too_large("mx4_pack", k=w.shape[1])
     _check(_mx("ta_mx4_pack")(_stream(), _code(w.dtype), w.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), n, w.shape[1]))
     return out
 
@@ -2998,6 +3004,8 @@ def mx4_unpack(w: Mx4, out: torch.Tensor) -> torch.Tensor:
     if tuple(out.shape) != w.shape:
         raise KernelError(f"mx4_unpack: w {w.shape} out {tuple(out.shape)}")
     _here("mx4_unpack", out, w.codes)
+    if w.shape[1] >> 31:
+        _too_large("mx4_unpack", k=w.shape[1])
     _check(_mx("ta_mx4_unpack")(_stream(), _code(out.dtype), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ld, n, w.shape[1]))
     return out
 
@@ -3010,6 +3018,8 @@ def mx8_pack(x: torch.Tensor, out: Mx8) -> Mx8:
     if tuple(x.shape) != out.shape:
         raise KernelError(f"mx8_pack: x {tuple(x.shape)} out {out.shape}")
     _here("mx8_pack", x, out.codes)
+    if x.shape[1] >> 31:
+        _too_large("mx8_pack", k=x.shape[1])
     _check(_mx("ta_mx8_pack")(_stream(), _code(x.dtype), x.data_ptr(), ld, out.codes.data_ptr(), out.scales.data_ptr(), m, x.shape[1]))
     return out
 
@@ -3026,6 +3036,8 @@ def swiglu_mx8(gate_up: torch.Tensor, out: Mx8, bias: Optional[torch.Tensor] = N
     ld, inner = gate_up.stride()
     if inner != 1:
         _rows2d(gate_up, "gate_up")
+    if d >> 31:
+        _too_large("swiglu_mx8", d=d)
     rc = _mx("ta_swiglu_mx8")(torch._C._cuda_getCurrentRawStream(at), _code(gate_up.dtype), gate_up.data_ptr(), ld,
                               None if bias is None else bias.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d)
     if rc:
@@ -3036,8 +3048,8 @@ def swiglu_mx8(gate_up: torch.Tensor, out: Mx8, bias: Optional[torch.Tensor] = N
 def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8, delta: Optional[torch.Tensor] = None,
                     delta_bias: Optional[torch.Tensor] = None, stream: Optional[torch.Tensor] = None) -> Mx8:
     """``add_rmsnorm`` with the normed rows left in 8 bits: v = x + delta + delta_bias goes back to x (to ``stream`` where one
-    is given, which then gets v also when nothing is added), rmsnorm(v) * weight to out. delta float32 or bfloat16 [m, d], or
-    [planes, m, d] whose planes are added in order."""
+    is given, which then gets v also when nothing is added), rmsnorm(v) * weight to out, summed and normed in 64 bits (rows of
+    more than 32,768: from v as stored). delta float32 or bfloat16 [m, d], or [planes, m, d] whose planes are added in order."""
     m, d = out.shape
     at = torch._C._cuda_getDevice()
     code = planes = dp = 0
@@ -3065,6 +3077,8 @@ def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8,
                           f"stream {None if stream is None else tuple(stream.shape)}")
     if m == 0:
         return out
+    if (m | d | planes) >> 31:
+        _too_large("add_rmsnorm_mx8", rows=m, d=d, planes=planes)
     rc = _mx("ta_add_rmsnorm_mx8")(torch._C._cuda_getCurrentRawStream(at), code, x.data_ptr(), dp or None, planes,
                                    None if delta_bias is None else delta_bias.data_ptr(), weight.data_ptr(), eps,
                                    None if stream is None else stream.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), m, d)
@@ -3074,11 +3088,30 @@ def add_rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Mx8,
 
 
 MX4_MAX_ROWS = 64       # bfloat16 rows that ``gemm_mx4`` takes (ta_mx4_max_rows)
-MX8_FEW_ROWS = 64       # 8-bit rows up to which it goes without scratch (MX_FEW_ROWS8 of csrc/mx_gemm.hip)
+_mx_scratch_sizes = {}
+
+
+def gemm_mx4_scratch(eight: bool, swiglu: bool, rows: int, n: int, k: int, aligned: bool = True) -> int:
+    """Bytes of scratch that ``gemm_mx4`` allocates for a call (n: columns of the result; aligned: scales on 16 bytes)."""
+    key = (eight, swiglu, rows, n, k, aligned)
+    need = _mx_scratch_sizes.get(key)
+    if need is None:
+        if (rows | n | k) >> 31:
+            _too_large("gemm_mx4_scratch", rows=rows, n=n, k=k)
+        f = library().ta_gemm_mx4_scratch
+        f.restype = c_longlong
+        if len(_mx_scratch_sizes) > 4096:
+            _mx_scratch_sizes.clear()
+        need = _mx_scratch_sizes[key] = int(f(c_int(eight), c_int(swiglu), c_int(rows), c_int(n), c_int(k), c_int(aligned)))
+    return need
+
+
+MX_FEW_ROWS = 16        # rows up to which no call needs any
 
 
 def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, swiglu: bool = False) -> torch.Tensor:
-    """out = a @ w.T (+ bias) with 4-bit weights, sums in float32.
+    """out = a @ w.T (+ bias) with 4-bit weights, sums in float32. k up to 8,388,608, rows of a bfloat16 ``a`` up to 16,777,216 values
+    apart, as many columns as one launch has threads for (below 2^30).
 
     a bfloat16, at most ``MX4_MAX_ROWS`` rows (more: ``mx4_unpack`` and a product of many bfloat16 rows): the weights enter with
     their exact values (one of 2^128 and more, which bfloat16 does not hold, as an infinity), out float32 or bfloat16. swiglu: w
@@ -3113,18 +3146,27 @@ def gemm_mx4(a, w: Mx4, out: torch.Tensor, bias: Optional[torch.Tensor] = None, 
         _rows2d(x, "a"); _rows2d(out, "out")
     if m == 0 or cols == 0:
         return out
+    if (m | n | k) >> 31:
+        _too_large("gemm_mx4", rows=m, n=n, k=k)
+    if swiglu and MX_FEW_ROWS < m <= MX4_MAX_ROWS and (n + 256) * (k // 2) >> 32:
+        # a tile counts from its gates to their ups in 32 bits: rows in the groups whose kernel has an address for either
+        for first in range(0, m, MX_FEW_ROWS):
+            gemm_mx4(a[first:first + MX_FEW_ROWS], w, out[first:first + MX_FEW_ROWS], bias, True)
+        return out
+    xs, ws = a.scales.data_ptr() if eight else 0, w.scales.data_ptr()
+    scratch = need = 0
+    if m > MX_FEW_ROWS:
+        need = gemm_mx4_scratch(eight, swiglu, m, cols, k, (xs | ws) % 16 == 0)
+        if need:        # the allocator's, so that calls on two streams, or two recorded graphs, do not share it
+            room = torch.empty(need, dtype=torch.uint8, device=out.device)
+            scratch = room.data_ptr()
     stream, bp = torch._C._cuda_getCurrentRawStream(at), None if bias is None else bias.data_ptr()
-    if not eight:
-        rc = _mx("ta_gemm_mx4")(stream, 0 if wide else 1, 1 if swiglu else 0, x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(),
-                                bp, out.data_ptr(), ldo, m, cols, k)
+    if eight:
+        rc = _mx("ta_gemm_mx4_mx8")(stream, x.data_ptr(), xs, w.codes.data_ptr(), ws, bp, out.data_ptr(), ldo, m, cols, k, scratch or None,
+                                    need)
     else:
-        xs, ws = a.scales.data_ptr(), w.scales.data_ptr()
-        scratch, need = None, 0
-        if m > MX8_FEW_ROWS and (k % 512 or (xs | ws) % 16):    # scales whose rows are off 16 bytes are laid out again
-            need = (m + n) * (-(-k // 512) * 16)
-            scratch = torch.empty(need, dtype=torch.uint8, device=out.device)
-        rc = _mx("ta_gemm_mx4_mx8")(stream, x.data_ptr(), xs, w.codes.data_ptr(), ws, bp, out.data_ptr(), ldo, m, cols, k,
-                                    None if scratch is None else scratch.data_ptr(), need)
+        rc = _mx("ta_gemm_mx4")(stream, 0 if wide else 1, 1 if swiglu else 0, x.data_ptr(), ldx, w.codes.data_ptr(), ws, bp, out.data_ptr(),
+                                ldo, m, cols, k, scratch or None, need)
     if rc:
         _check(rc)
     return out
